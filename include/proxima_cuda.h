@@ -749,6 +749,81 @@ uint32_t pxc_sq_last_retried(const pxc_sq* h);
  * buffer and were answered by the exact chunked fallback. */
 uint32_t pxc_sq_last_fallback(const pxc_sq* h);
 
+/* ---- BlockQuantizer: 8-bit floating codes with a scale for each block of 128 ----
+ * No counterpart in the reference, whose 8-bit codes are ranges per component
+ * (ScalarQuantizer above) and codewords (ProductQuantizer). A row of `dim`
+ * components is held as e4m3 codes and, for each block of 128 components (the
+ * last may be shorter), one scale 2^s kept as the byte s + 127 (E8M0). The
+ * encoder takes the smallest s >= -126 for which the block's largest finite
+ * magnitude is at most 448 * 2^s (s = 0 for a block without one) and rounds
+ * value / 2^s to e4m3, nearest, ties to even; an infinity becomes +-448 and a
+ * NaN stays one.
+ *
+ * All entry points: 1 <= dim <= 2^20, at most 2^31 - 257 rows. The device forms
+ * are ordered on `stream` (NULL: the context's), neither allocate nor wait and
+ * may be captured into a graph; calls on one context may run concurrently. A
+ * failure that only the device sees (offsets that are no partition, a wait that
+ * ran out) leaves that call's outputs undefined, writes nothing outside them, and is
+ * reported by a later pxc_bq_* call on the context, once: PXC_CONFIGURATION
+ * ("offsets") or PXC_TIMEOUT. The host forms report their own. */
+#define PXC_DTYPE_F32 0
+#define PXC_DTYPE_F16 1
+#define PXC_DTYPE_BF16 2
+/* Encoded rows: row r's codes are bytes codes[r * ld ..+ dim), its scales bytes
+ * scales[r * sld ..+ ceil(dim / 128)), in buffers of rows * ld and rows * sld
+ * bytes. ld >= dim is a multiple of 16, sld >= ceil(dim / 128) a multiple of 4;
+ * in device memory `codes` is 16-byte aligned and `scales` 4-byte aligned. */
+typedef struct pxc_bq_rows {
+  uint8_t* codes;
+  uint8_t* scales;
+  uint64_t rows;
+  uint64_t ld;
+  uint64_t sld;
+} pxc_bq_rows;
+/* Encodes out->rows HOST vectors of `dim` components, `stride` components apart. Code
+ * bytes up to the next multiple of 16 and scale bytes up to the next multiple
+ * of 4 are zero; further pitch bytes are left as they were. */
+pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint64_t stride, uint32_t dim,
+                         const pxc_bq_rows* out, pxc_error* err);
+/* Same with DEVICE vectors, codes and scales. */
+pxc_status pxc_bq_encode_device(pxc_ctx* ctx, const void* d_vectors, int32_t dtype, uint64_t stride, uint32_t dim,
+                                const pxc_bq_rows* d_out, void* stream, pxc_error* err);
+/* The vectors that the rows stand for: code * 2^s, rounded once to `dtype`;
+ * `stride` components from row to row. HOST buffers. */
+pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, void* out, int32_t dtype,
+                         uint64_t stride, pxc_error* err);
+/* Same with DEVICE buffers. */
+pxc_status pxc_bq_decode_device(pxc_ctx* ctx, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out, int32_t dtype,
+                                uint64_t stride, void* stream, pxc_error* err);
+/* The dot product of every pair of encoded rows: out[q * stride + r] = queries[q] .
+ * base[r], summed in f32 and rounded once to `dtype`; stride >= base->rows. HOST buffers. */
+pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq_rows* base, uint32_t dim, void* out,
+                          int32_t dtype, uint64_t stride, pxc_error* err);
+/* Same with DEVICE buffers. */
+pxc_status pxc_bq_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base, uint32_t dim,
+                                 void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err);
+/* The product of each of `groups` ragged groups: group g pairs the queries
+ * [query_offsets[g], query_offsets[g + 1]) with the base rows [base_offsets[g],
+ * base_offsets[g + 1]). Offsets rise and stay within the rows; either side of
+ * a group may be empty.
+ *   base_offsets given: `out` holds the groups' m_g x n_g matrices one after the
+ *     other, row-major, without gaps; `size` is the room in `out`, in values.
+ *   base_offsets NULL: base->rows is a multiple of `groups`, each group has
+ *     n = base->rows / groups rows, and query q writes out[q * n ..+ n); size >=
+ *     queries->rows * n. Rows of `out` for queries in no group are left as they were.
+ * HOST buffers. */
+pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const int64_t* query_offsets,
+                                  const pxc_bq_rows* base, const int64_t* base_offsets, uint32_t groups, uint32_t dim,
+                                  void* out, int32_t dtype, uint64_t size, pxc_error* err);
+/* Same with DEVICE buffers, the offsets (groups + 1 each) among them. */
+pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const int64_t* d_query_offsets,
+                                         const pxc_bq_rows* d_base, const int64_t* d_base_offsets, uint32_t groups,
+                                         uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
+                                         pxc_error* err);
+/* Waits for `stream` (NULL: the context's) and reports a failure that the device
+ * forms left, as above. */
+pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err);
+
 #ifdef __cplusplus
 }
 #endif

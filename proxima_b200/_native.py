@@ -116,6 +116,13 @@ class PxcOperand(C.Structure):
     _fields_ = [("tag", C.c_uint32), ("reserved", C.c_uint32), ("value", C.c_int64)]
 
 
+class PxcBqRows(C.Structure):
+    """pxc_bq_rows: block-quantised rows (codes, scales and their pitches)."""
+
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint64), ("ld", C.c_uint64),
+                ("sld", C.c_uint64)]
+
+
 class PxcIntRange(C.Structure):
     """pxc_int_range: lo <= value <= hi on an integer metadata column."""
 
@@ -256,6 +263,23 @@ SIGNATURES: dict[str, tuple] = {
     "pxc_sq_last_accepted": (C.c_uint64, [vp]),
     "pxc_sq_last_fallback": (C.c_uint32, [vp]),
     "pxc_sq_last_retried": (C.c_uint32, [vp]),
+    "pxc_bq_encode": (C.c_int32, [vp, vp, C.c_int32, C.c_uint64, C.c_uint32, C.POINTER(PxcBqRows),
+                                  C.POINTER(PxcError)]),
+    "pxc_bq_encode_device": (C.c_int32, [vp, vp, C.c_int32, C.c_uint64, C.c_uint32, C.POINTER(PxcBqRows), vp,
+                                         C.POINTER(PxcError)]),
+    "pxc_bq_decode": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32, C.c_uint64,
+                                  C.POINTER(PxcError)]),
+    "pxc_bq_decode_device": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32, C.c_uint64, vp,
+                                         C.POINTER(PxcError)]),
+    "pxc_bq_product": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32,
+                                   C.c_uint64, C.POINTER(PxcError)]),
+    "pxc_bq_product_device": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32,
+                                          C.c_uint64, vp, C.POINTER(PxcError)]),
+    "pxc_bq_grouped_product": (C.c_int32, [vp, C.POINTER(PxcBqRows), vp, C.POINTER(PxcBqRows), vp, C.c_uint32,
+                                           C.c_uint32, vp, C.c_int32, C.c_uint64, C.POINTER(PxcError)]),
+    "pxc_bq_grouped_product_device": (C.c_int32, [vp, C.POINTER(PxcBqRows), vp, C.POINTER(PxcBqRows), vp, C.c_uint32,
+                                                  C.c_uint32, vp, C.c_int32, C.c_uint64, vp, C.POINTER(PxcError)]),
+    "pxc_bq_check": (C.c_int32, [vp, vp, C.POINTER(PxcError)]),
 }
 
 _lib = None

@@ -1,0 +1,516 @@
+// bq.cu — the block quantiser (pxc_bq_*): encode, decode, the product of two sets of
+// encoded rows, and the product grouped by ragged lists.
+#include <algorithm>
+#include <type_traits>
+
+#include "bq.cuh"
+
+namespace pxc {
+namespace bq {
+
+constexpr uint64_t MAX_ROWS = (uint64_t(1) << 31) - 257;  // row numbers and tile ends fit an int32
+constexpr uint32_t MAX_DIM = 1u << 20;
+constexpr uint64_t MAX_SIZE = uint64_t(1) << 48;  // values in an output: offsets of them cannot overflow
+
+static uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
+static uint32_t blocks_of(uint32_t dim) { return (dim + BLOCK - 1) / BLOCK; }
+
+// ---- encode ----
+// A warp per block of 128: four components a lane, the largest magnitude by one warp reduction,
+// one packed store of the four codes.
+template <class T>
+__global__ void __launch_bounds__(256)
+    encode_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
+                  uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5);
+  const uint64_t total = rows * blocks;
+  const uint32_t code_end = (dim + 15) / 16 * 16;
+  for (uint64_t w = static_cast<uint64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps) {
+    const uint64_t r = w / blocks;
+    const uint32_t j = static_cast<uint32_t>(w - r * blocks);
+    const uint32_t c0 = j * BLOCK + lane * 4;
+    const T* row = x + r * stride;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c0 + i < dim ? to_f32<T>(row[c0 + i]) : 0.0f;
+    const uint32_t top = max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
+    const uint32_t byte = scale_byte(__reduce_max_sync(0xFFFFFFFFu, top));
+    const float f = inverse_scale(byte);
+    if (c0 < code_end)
+      *reinterpret_cast<uint32_t*>(codes + r * ld + c0) = to_codes(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+    if (lane == 0) {
+      uint8_t* s = scales + r * sld;
+      s[j] = static_cast<uint8_t>(byte);
+      if (j + 1 == blocks)
+        for (uint32_t k = blocks; k & 3; ++k) s[k] = 0;
+    }
+  }
+}
+
+// ---- decode ----
+template <class T>
+__global__ void __launch_bounds__(256)
+    decode_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales, uint64_t sld,
+                  uint64_t rows, uint32_t dim, T* __restrict__ out, uint64_t stride) {
+  const uint32_t quads = (dim + 3) / 4;
+  const uint64_t total = rows * quads;
+  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
+    const uint64_t r = i / quads;
+    const uint32_t c0 = static_cast<uint32_t>(i - r * quads) * 4;
+    const uint32_t four = *reinterpret_cast<const uint32_t*>(codes + r * ld + c0);
+    const float f = scale_value(scales[r * sld + c0 / BLOCK]);
+    const float2 a = from_codes(four & 0xFFFFu), b = from_codes(four >> 16);
+    const float v[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
+    T* dst = out + r * stride + c0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c0 + k < dim) dst[k] = from_f32<T>(v[k]);
+  }
+}
+
+// ---- product ----
+struct Operand {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  uint64_t ld, sld;
+};
+
+// 64 queries x 64 rows per block and 16 values a thread, 32 components at a time through shared
+// memory as f32.
+constexpr uint32_t PT = 64, PK = 32;
+template <class T>
+__global__ void __launch_bounds__(256) product_kernel(Operand q, Operand b, uint32_t dim, Groups groups, T* out) {
+  __shared__ float sq[PK][PT + 4], sb[PK][PT + 4];
+  __shared__ Tile tile;
+  __shared__ uint32_t found;
+  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  Walk<PT, PT> walk(groups, threadIdx.x & 31);
+  for (uint64_t t = blockIdx.x;; t += gridDim.x) {
+    if (threadIdx.x < 32) {
+      Tile mine;
+      const bool any = walk.find(t, mine);
+      if (threadIdx.x == 0) {
+        found = any;
+        if (any) tile = mine;
+      }
+    }
+    __syncthreads();
+    if (!found) return;
+    const Tile w = tile;
+    float acc[4][4] = {};
+    for (uint32_t k0 = 0; k0 < dim; k0 += PK) {
+      // 64 rows x 8 quads of codes on either side: two quads a thread
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t i = threadIdx.x + h * 256, row = i >> 3, c = k0 + (i & 7) * 4;
+        float2 lo = {0, 0}, hi = {0, 0};
+        if (row < w.queries && c < dim) {
+          const uint64_t r = w.q0 + row;
+          const uint32_t four = *reinterpret_cast<const uint32_t*>(q.codes + r * q.ld + c);
+          const float f = scale_value(q.scales[r * q.sld + c / BLOCK]);
+          lo = from_codes(four & 0xFFFFu), hi = from_codes(four >> 16);
+          lo.x *= f, lo.y *= f, hi.x *= f, hi.y *= f;
+        }
+        const uint32_t kk = (i & 7) * 4;
+        sq[kk][row] = lo.x, sq[kk + 1][row] = c + 1 < dim ? lo.y : 0.f;
+        sq[kk + 2][row] = c + 2 < dim ? hi.x : 0.f, sq[kk + 3][row] = c + 3 < dim ? hi.y : 0.f;
+        lo = {0, 0}, hi = {0, 0};
+        if (row < w.rows && c < dim) {
+          const uint64_t r = w.b0 + row;
+          const uint32_t four = *reinterpret_cast<const uint32_t*>(b.codes + r * b.ld + c);
+          const float f = scale_value(b.scales[r * b.sld + c / BLOCK]);
+          lo = from_codes(four & 0xFFFFu), hi = from_codes(four >> 16);
+          lo.x *= f, lo.y *= f, hi.x *= f, hi.y *= f;
+        }
+        sb[kk][row] = lo.x, sb[kk + 1][row] = c + 1 < dim ? lo.y : 0.f;
+        sb[kk + 2][row] = c + 2 < dim ? hi.x : 0.f, sb[kk + 3][row] = c + 3 < dim ? hi.y : 0.f;
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (uint32_t k = 0; k < PK; ++k) {
+        float a[4], c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = sq[k][ty * 4 + i], c[i] = sb[k][tx + 16 * i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * c[j];
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t y = ty * 4 + i, x = tx + 16 * j;
+        if (y < w.queries && x < w.rows) out[w.at + y * w.stride + x] = from_f32<T>(acc[i][j]);
+      }
+  }
+}
+
+// ---- host ----
+static void check_common(const pxc_ctx* ctx, uint32_t dim, int32_t dtype) {
+  PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
+  PXC_CONFIG(dim >= 1 && dim <= MAX_DIM, "dim", dim, "must be between 1 and 1048576");
+  PXC_CONFIG(dtype == PXC_DTYPE_F32 || dtype == PXC_DTYPE_F16 || dtype == PXC_DTYPE_BF16, "dtype", dtype,
+             "must be f32, f16 or bf16");
+}
+
+// Device rows are read by wide loads and tensor maps; host rows are copied, at any alignment.
+static void check_rows(const pxc_bq_rows* r, uint32_t dim, const char* name, bool device) {
+  PXC_CONFIG(r != nullptr, name, 0, "null rows");
+  PXC_CONFIG(r->rows <= MAX_ROWS, name, r->rows, "at most 2^31 - 257 rows");
+  if (r->rows == 0) return;
+  PXC_CONFIG(r->codes != nullptr && r->scales != nullptr, name, 0, "null codes or scales");
+  PXC_CONFIG(!device || (reinterpret_cast<uintptr_t>(r->codes) & 15) == 0, name, reinterpret_cast<uintptr_t>(r->codes),
+             "codes must be 16-byte aligned");
+  PXC_CONFIG(!device || (reinterpret_cast<uintptr_t>(r->scales) & 3) == 0, name, reinterpret_cast<uintptr_t>(r->scales),
+             "scales must be 4-byte aligned");
+  PXC_CONFIG(r->ld >= dim && (r->ld & 15) == 0 && r->ld < (uint64_t(1) << 32), "ld", r->ld,
+             "the code pitch must be a multiple of 16, at least dim and below 2^32");
+  PXC_CONFIG(r->sld >= blocks_of(dim) && (r->sld & 3) == 0 && r->sld < (uint64_t(1) << 32), "sld", r->sld,
+             "the scale pitch must be a multiple of 4, at least ceil(dim / 128) and below 2^32");
+}
+
+// Reports a failure that an earlier device call left, once.
+static void take_fault(pxc_ctx* ctx) {
+  bool set[FAULT_WORDS];
+  for (uint32_t i = 0; i < FAULT_WORDS; ++i)
+    set[i] = __atomic_load_n(ctx->bq_faults + i, __ATOMIC_RELAXED) != 0 &&
+             __atomic_exchange_n(ctx->bq_faults + i, 0u, __ATOMIC_RELAXED) != 0;
+  if (set[FAULT_TIMEOUT])
+    throw make_failure(PXC_TIMEOUT, 0, 0, nullptr, "a device-side wait of a block product ran out");
+  if (set[FAULT_OFFSETS])
+    throw make_failure(PXC_CONFIGURATION, 0, 0, "offsets",
+                       "a grouped product's offsets fell, left the rows, or did not fit the output");
+}
+
+static void count_launch(pxc_ctx* ctx) { __atomic_fetch_add(&ctx->launches, 1ull, __ATOMIC_RELAXED); }
+
+static size_t size_of(int32_t dtype) { return dtype == PXC_DTYPE_F32 ? 4 : 2; }
+
+template <class F>
+static void with_type(int32_t dtype, F&& f) {
+  if (dtype == PXC_DTYPE_F32)
+    f(static_cast<float*>(nullptr));
+  else if (dtype == PXC_DTYPE_F16)
+    f(static_cast<__half*>(nullptr));
+  else
+    f(static_cast<__nv_bfloat16*>(nullptr));
+}
+
+static void encode(pxc_ctx* ctx, const void* x, int32_t dtype, uint64_t stride, uint32_t dim, const pxc_bq_rows& out,
+                   cudaStream_t s) {
+  const uint32_t blocks = blocks_of(dim);
+  const unsigned grid =
+      static_cast<unsigned>(std::min<uint64_t>((out.rows * blocks + 7) / 8, static_cast<uint64_t>(ctx->sm_count) * 32));
+  with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    encode_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(x), stride, out.rows, dim, blocks, out.codes, out.ld,
+                                          out.scales, out.sld);
+  });
+  PXC_CUDA(cudaGetLastError());
+  count_launch(ctx);
+}
+
+static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out, int32_t dtype, uint64_t stride,
+                   cudaStream_t s) {
+  const uint64_t quads = in.rows * ((dim + 3) / 4);
+  const unsigned grid =
+      static_cast<unsigned>(std::min<uint64_t>((quads + 255) / 256, static_cast<uint64_t>(ctx->sm_count) * 32));
+  with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    decode_kernel<T><<<grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, static_cast<T*>(out), stride);
+  });
+  PXC_CUDA(cudaGetLastError());
+  count_launch(ctx);
+}
+
+static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, Groups g, void* out,
+                    int32_t dtype, cudaStream_t s) {
+  g.nq = q.rows;
+  g.nb = b.rows;
+  g.faults = ctx->bq_faults;
+  with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    product_kernel<T><<<ctx->sm_count * 4, 256, 0, s>>>(Operand{q.codes, q.scales, q.ld, q.sld},
+                                                        Operand{b.codes, b.scales, b.ld, b.sld}, dim, g,
+                                                        static_cast<T*>(out));
+  });
+  PXC_CUDA(cudaGetLastError());
+  count_launch(ctx);
+}
+
+static void check_vectors(const void* x, int32_t dtype, uint64_t stride, uint32_t dim, const char* name) {
+  PXC_CONFIG(x != nullptr, name, 0, "null buffer");
+  PXC_CONFIG(reinterpret_cast<uintptr_t>(x) % size_of(dtype) == 0, name, reinterpret_cast<uintptr_t>(x),
+             "not aligned to its type");
+  PXC_CONFIG(stride >= dim && stride < (uint64_t(1) << 32), "stride", stride, "must be at least dim and below 2^32");
+}
+
+static void check_product(const pxc_bq_rows* q, const pxc_bq_rows* b, uint32_t dim, const void* out, int32_t dtype,
+                          uint64_t stride, bool device) {
+  check_rows(q, dim, "queries", device);
+  check_rows(b, dim, "base", device);
+  if (q->rows == 0 || b->rows == 0) return;
+  PXC_CONFIG(out != nullptr && reinterpret_cast<uintptr_t>(out) % size_of(dtype) == 0, "out",
+             reinterpret_cast<uintptr_t>(out), "null or not aligned to its type");
+  PXC_CONFIG(stride >= b->rows && stride <= MAX_SIZE / q->rows, "stride", stride,
+             "must be at least the base rows, and the output at most 2^48 values");
+}
+
+// The even form's rows per group.
+static uint64_t check_grouped(const pxc_bq_rows* q, const void* qo, const pxc_bq_rows* b, const void* bo, uint32_t groups,
+                              uint32_t dim, const void* out, int32_t dtype, uint64_t size, bool device) {
+  check_rows(q, dim, "queries", device);
+  check_rows(b, dim, "base", device);
+  PXC_CONFIG(groups >= 1 && groups <= (1u << 24), "groups", groups, "must be between 1 and 16777216");
+  PXC_CONFIG(qo != nullptr, "offsets", 0, "null query offsets");
+  PXC_CONFIG(size <= MAX_SIZE, "size", size, "at most 2^48 values");
+  PXC_CONFIG(size == 0 || (out != nullptr && reinterpret_cast<uintptr_t>(out) % size_of(dtype) == 0), "out",
+             reinterpret_cast<uintptr_t>(out), "null or not aligned to its type");
+  if (bo) return 0;
+  PXC_CONFIG(b->rows % groups == 0, "base", b->rows, "without base offsets the rows must be a multiple of the groups");
+  const uint64_t each = b->rows / groups;
+  PXC_CONFIG(q->rows == 0 || each <= MAX_SIZE / q->rows, "base", b->rows, "the output is at most 2^48 values");
+  PXC_CONFIG(size >= q->rows * each, "size", size, "smaller than the queries times a group's rows");
+  return each;
+}
+
+// Device copies of host rows, with the pitches that the kernels want.
+struct Staged {
+  DBuf<uint8_t> codes, scales;
+  pxc_bq_rows d{};
+  void make(uint64_t rows, uint32_t dim) {
+    d.rows = rows;
+    d.ld = up(dim, 16);
+    d.sld = up(blocks_of(dim), 4);
+    codes.reserve(rows * d.ld);
+    scales.reserve(rows * d.sld);
+    d.codes = codes.p;
+    d.scales = scales.p;
+  }
+  void load(const pxc_bq_rows& h, uint32_t dim, cudaStream_t s) {
+    make(h.rows, dim);
+    if (h.rows == 0) return;
+    PXC_CUDA(cudaMemcpy2DAsync(d.codes, d.ld, h.codes, h.ld, dim, h.rows, cudaMemcpyHostToDevice, s));
+    PXC_CUDA(cudaMemcpy2DAsync(d.scales, d.sld, h.scales, h.sld, blocks_of(dim), h.rows, cudaMemcpyHostToDevice, s));
+  }
+};
+
+static void check_host_offsets(const int64_t* o, uint32_t groups, uint64_t rows) {
+  for (uint32_t g = 0; g < groups; ++g)
+    PXC_CONFIG(o[g] >= 0 && o[g + 1] >= o[g] && static_cast<uint64_t>(o[g + 1]) <= rows, "offsets", g,
+               "offsets must rise and stay within the rows");
+}
+
+static void finish(pxc_ctx* ctx, cudaStream_t s) {
+  PXC_CUDA(cudaStreamSynchronize(s));
+  take_fault(ctx);
+}
+
+}  // namespace bq
+}  // namespace pxc
+
+using namespace pxc;
+
+extern "C" {
+
+pxc_status pxc_bq_encode_device(pxc_ctx* ctx, const void* d_vectors, int32_t dtype, uint64_t stride, uint32_t dim,
+                                const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_rows(d_out, dim, "out", true);
+    if (d_out->rows == 0) return;
+    bq::check_vectors(d_vectors, dtype, stride, dim, "vectors");
+    DeviceGuard g(ctx->device);
+    bq::encode(ctx, d_vectors, dtype, stride, dim, *d_out, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+  });
+}
+
+pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint64_t stride, uint32_t dim,
+                         const pxc_bq_rows* out, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_rows(out, dim, "out", false);
+    if (out->rows == 0) return;
+    bq::check_vectors(vectors, dtype, stride, dim, "vectors");
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    DeviceGuard g(ctx->device);
+    cudaStream_t s = ctx->stream;
+    const size_t es = bq::size_of(dtype);
+    DBuf<uint8_t> x;
+    x.reserve(out->rows * dim * es);
+    bq::Staged c;
+    c.make(out->rows, dim);
+    PXC_CUDA(cudaMemcpy2DAsync(x.p, dim * es, vectors, stride * es, dim * es, out->rows, cudaMemcpyHostToDevice, s));
+    bq::encode(ctx, x.p, dtype, dim, dim, c.d, s);
+    PXC_CUDA(cudaMemcpy2DAsync(out->codes, out->ld, c.d.codes, c.d.ld, c.d.ld, out->rows, cudaMemcpyDeviceToHost, s));
+    PXC_CUDA(cudaMemcpy2DAsync(out->scales, out->sld, c.d.scales, c.d.sld, c.d.sld, out->rows, cudaMemcpyDeviceToHost, s));
+    PXC_CUDA(cudaStreamSynchronize(s));
+  });
+}
+
+pxc_status pxc_bq_decode_device(pxc_ctx* ctx, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out, int32_t dtype,
+                                uint64_t stride, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_rows(d_rows, dim, "rows", true);
+    if (d_rows->rows == 0) return;
+    bq::check_vectors(d_out, dtype, stride, dim, "out");
+    DeviceGuard g(ctx->device);
+    bq::decode(ctx, *d_rows, dim, d_out, dtype, stride, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+  });
+}
+
+pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, void* out, int32_t dtype, uint64_t stride,
+                         pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_rows(rows, dim, "rows", false);
+    if (rows->rows == 0) return;
+    bq::check_vectors(out, dtype, stride, dim, "out");
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    DeviceGuard g(ctx->device);
+    cudaStream_t s = ctx->stream;
+    const size_t es = bq::size_of(dtype);
+    bq::Staged c;
+    c.load(*rows, dim, s);
+    DBuf<uint8_t> x;
+    x.reserve(rows->rows * dim * es);
+    bq::decode(ctx, c.d, dim, x.p, dtype, dim, s);
+    PXC_CUDA(cudaMemcpy2DAsync(out, stride * es, x.p, dim * es, dim * es, rows->rows, cudaMemcpyDeviceToHost, s));
+    PXC_CUDA(cudaStreamSynchronize(s));
+  });
+}
+
+pxc_status pxc_bq_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base, uint32_t dim,
+                                 void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_product(d_queries, d_base, dim, d_out, dtype, stride, true);
+    if (d_queries->rows == 0 || d_base->rows == 0) return;
+    DeviceGuard g(ctx->device);
+    bq::Groups groups{};
+    groups.groups = 1;
+    groups.n_each = d_base->rows;
+    groups.stride = stride;
+    bq::product(ctx, *d_queries, *d_base, dim, groups, d_out, dtype,
+                stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+  });
+}
+
+pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq_rows* base, uint32_t dim, void* out,
+                          int32_t dtype, uint64_t stride, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    bq::check_product(queries, base, dim, out, dtype, stride, false);
+    if (queries->rows == 0 || base->rows == 0) return;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    DeviceGuard g(ctx->device);
+    cudaStream_t s = ctx->stream;
+    const size_t es = bq::size_of(dtype);
+    bq::Staged q, b;
+    q.load(*queries, dim, s);
+    b.load(*base, dim, s);
+    DBuf<uint8_t> o;
+    o.reserve(queries->rows * base->rows * es);
+    bq::Groups groups{};
+    groups.groups = 1;
+    groups.n_each = groups.stride = base->rows;
+    bq::product(ctx, q.d, b.d, dim, groups, o.p, dtype, s);
+    PXC_CUDA(cudaMemcpy2DAsync(out, stride * es, o.p, base->rows * es, base->rows * es, queries->rows,
+                               cudaMemcpyDeviceToHost, s));
+    bq::finish(ctx, s);
+  });
+}
+
+pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const int64_t* d_query_offsets,
+                                         const pxc_bq_rows* d_base, const int64_t* d_base_offsets, uint32_t groups,
+                                         uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
+                                         pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    const uint64_t each =
+        bq::check_grouped(d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim, d_out, dtype, size, true);
+    if (d_queries->rows == 0 || d_base->rows == 0 || size == 0) return;
+    DeviceGuard g(ctx->device);
+    bq::Groups gr{};
+    gr.q_offsets = d_query_offsets;
+    gr.b_offsets = d_base_offsets;
+    gr.groups = groups;
+    gr.n_each = gr.stride = each;
+    gr.size = size;
+    bq::product(ctx, *d_queries, *d_base, dim, gr, d_out, dtype,
+                stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+  });
+}
+
+pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const int64_t* query_offsets,
+                                  const pxc_bq_rows* base, const int64_t* base_offsets, uint32_t groups, uint32_t dim,
+                                  void* out, int32_t dtype, uint64_t size, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_common(ctx, dim, dtype);
+    bq::take_fault(ctx);
+    const uint64_t each = bq::check_grouped(queries, query_offsets, base, base_offsets, groups, dim, out, dtype, size, false);
+    bq::check_host_offsets(query_offsets, groups, queries->rows);
+    uint64_t need = queries->rows * each;
+    if (base_offsets) {
+      bq::check_host_offsets(base_offsets, groups, base->rows);
+      need = 0;
+      for (uint32_t g = 0; g < groups; ++g) {
+        need += static_cast<uint64_t>(query_offsets[g + 1] - query_offsets[g]) *
+                static_cast<uint64_t>(base_offsets[g + 1] - base_offsets[g]);
+        PXC_CONFIG(need <= size, "size", size, "smaller than the groups' matrices together");
+      }
+    }
+    if (need == 0) return;
+    std::lock_guard<std::mutex> lock(ctx->mu);
+    DeviceGuard g(ctx->device);
+    cudaStream_t s = ctx->stream;
+    const size_t es = bq::size_of(dtype);
+    bq::Staged q, b;
+    q.load(*queries, dim, s);
+    b.load(*base, dim, s);
+    DBuf<int64_t> off;
+    off.reserve(2 * (size_t(groups) + 1));
+    PXC_CUDA(cudaMemcpyAsync(off.p, query_offsets, (size_t(groups) + 1) * 8, cudaMemcpyHostToDevice, s));
+    if (base_offsets)
+      PXC_CUDA(cudaMemcpyAsync(off.p + groups + 1, base_offsets, (size_t(groups) + 1) * 8, cudaMemcpyHostToDevice, s));
+    DBuf<uint8_t> o;
+    o.reserve(need * es);
+    // the even form leaves the rows of queries in no group as they were: only the others come back
+    const uint64_t first = base_offsets ? 0 : static_cast<uint64_t>(query_offsets[0]) * each;
+    const uint64_t count = base_offsets ? need : static_cast<uint64_t>(query_offsets[groups]) * each - first;
+    bq::Groups gr{};
+    gr.q_offsets = off.p;
+    gr.b_offsets = base_offsets ? off.p + groups + 1 : nullptr;
+    gr.groups = groups;
+    gr.n_each = gr.stride = each;
+    gr.size = need;
+    bq::product(ctx, q.d, b.d, dim, gr, o.p, dtype, s);
+    if (count)
+      PXC_CUDA(cudaMemcpyAsync(static_cast<uint8_t*>(out) + first * es, o.p + first * es, count * es,
+                               cudaMemcpyDeviceToHost, s));
+    bq::finish(ctx, s);
+  });
+}
+
+pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
+    DeviceGuard g(ctx->device);
+    bq::finish(ctx, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,218 @@
+// bq.cuh — block-quantised rows: the arithmetic of the codes and scales, and the walk over the
+// output tiles of a dense or grouped product.
+//
+// A block of 128 components with largest finite magnitude t has the scale 2^s, s the smallest
+// exponent >= -126 with t <= 448 * 2^s, kept as the byte s + 127 (E8M0). 448 = 1.75 * 2^8 is the
+// largest e4m3 value, so for t = 1.f * 2^(E - 127) the byte is E - 8, one more when 1.f > 1.75:
+// an integer rule on t's bits. Scaling by a power of two is exact, so a code carries one
+// rounding, that to e4m3.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace pxc {
+namespace bq {
+
+constexpr uint32_t BLOCK = 128;  // components per scale
+
+// Failures that only the device sees: a word each in pinned host memory, set by the kernel and
+// taken by the next call.
+enum Fault : uint32_t { FAULT_OFFSETS = 0, FAULT_TIMEOUT = 1, FAULT_WORDS = 2 };
+__device__ __forceinline__ void leave_fault(uint32_t* faults, Fault which) {
+  *reinterpret_cast<volatile uint32_t*>(faults + which) = 1;
+  __threadfence_system();
+}
+
+// ---- one block's scale ----
+// `top` holds the bits of the largest finite magnitude. Bytes are 1..247 (127 for top == 0), so
+// both 2^s and 2^-s are normal floats.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+  if (top == 0) return 127u;
+  const int32_t e = static_cast<int32_t>(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return static_cast<uint32_t>(max(e, 1));
+}
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^(byte - 127) for any E8M0 byte: 0 is the subnormal 2^-127, 255 is NaN.
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  if (byte == 0) return __uint_as_float(0x00400000u);
+  return byte == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
+}
+// Magnitude bits of a finite value, 0 for an infinity or NaN.
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+
+// Four values to four e4m3 codes, the first in the lowest byte: nearest, ties to even,
+// magnitudes above 448 (only infinities, after scaling) to 448, NaN to NaN.
+__device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+// Two codes to f32: every e4m3 value is a half.
+__device__ __forceinline__ float2 from_codes(uint32_t two) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two), __NV_E4M3)));
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// ---- the tiles of a product ----
+// A dense product is one group over all rows. Query offsets and base offsets are read where given
+// (`groups` + 1 each); without base offsets every group has n_each rows and the output is
+// indexed by query, else the groups' matrices follow one another.
+struct Groups {
+  const int64_t* q_offsets;  // NULL: dense
+  const int64_t* b_offsets;  // NULL: even
+  uint32_t groups;
+  uint64_t nq, nb;      // rows on either side
+  uint64_t n_each;      // even (and dense): base rows per group, and the output's row pitch is `stride`
+  uint64_t stride;
+  uint64_t size;        // room in the output, in values (ragged)
+  uint32_t* faults;
+};
+
+// One output tile: `queries` x `rows` values from (q0, b0), the first at out[at].
+struct Tile {
+  uint32_t q0, queries, b0, rows;
+  uint64_t at, stride;
+};
+
+// Walks the tiles in order, a warp at a time: lane i holds group chunk + i. Tiles are numbered
+// through the groups; find() is called with rising numbers, so that each chunk of 32 groups is
+// read once. Inside a group the queries come in panels of PANEL tiles, so that a panel's
+// queries stay in L2 while the base rows pass once.
+//
+// Every group is checked before it counts: its offsets rise and lie within the rows, and its
+// matrix ends within the output. One that fails counts as empty and leaves a fault, so
+// that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
+template <uint32_t TQ, uint32_t TB>
+struct Walk {
+  static constexpr uint32_t PANEL = 16;
+  const Groups& g;
+  const uint32_t lane;
+  uint32_t chunk = 0;
+  uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
+  uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
+  uint64_t q0 = 0, b0 = 0, m = 0, n = 0;
+
+  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id) : g(groups), lane(lane_id) { load(); }
+
+  __device__ __forceinline__ static uint64_t scan(uint64_t v, uint32_t lane) {
+#pragma unroll
+    for (uint32_t d = 1; d < 32; d <<= 1) {
+      const uint64_t u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      if (lane >= d) v += u;
+    }
+    return v;
+  }
+  __device__ __forceinline__ static uint64_t tiles_of(uint64_t m, uint64_t n) {
+    return ((m + TQ - 1) / TQ) * ((n + TB - 1) / TB);
+  }
+
+  __device__ __forceinline__ void load() {
+    const uint32_t i = chunk + lane;
+    q0 = b0 = m = n = 0;
+    if (i < g.groups) {
+      bool good = true;
+      if (g.q_offsets) {
+        const int64_t lo = g.q_offsets[i], hi = g.q_offsets[i + 1];
+        good = lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nq);
+        q0 = static_cast<uint64_t>(lo);
+        m = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
+      } else {
+        m = g.nq;
+      }
+      if (g.b_offsets) {
+        const int64_t lo = g.b_offsets[i], hi = g.b_offsets[i + 1];
+        good = good && lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nb);
+        b0 = static_cast<uint64_t>(lo);
+        n = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
+      } else {
+        b0 = i * g.n_each;
+        n = g.n_each;
+      }
+      if (!good) {
+        leave_fault(g.faults, FAULT_OFFSETS);
+        q0 = b0 = m = n = 0;
+      }
+    }
+    if (g.b_offsets) {
+      // m, n < 2^31 and size <= 2^48: with each term held to size + 1 no sum overflows, and one
+      // that is past the room stays past it for all groups behind
+      values_upto = scan(min(m * n, g.size + 1), lane);
+      if (m * n != 0 && values_before + values_upto > g.size) {
+        leave_fault(g.faults, FAULT_OFFSETS);
+        m = 0;
+      }
+    }
+    tiles_upto = scan(tiles_of(m, n), lane);
+  }
+
+  // Tile number t, or false when there are fewer. All lanes call and get the same answer.
+  __device__ __forceinline__ bool find(uint64_t t, Tile& out) {
+    for (;;) {
+      const uint64_t total = __shfl_sync(0xFFFFFFFFu, tiles_upto, 31);
+      if (t < tiles_before + total) break;
+      tiles_before += total;
+      values_before = min(values_before + __shfl_sync(0xFFFFFFFFu, values_upto, 31), uint64_t(1) << 60);
+      if (g.groups - chunk <= 32) {
+        chunk = g.groups;  // nothing behind: later calls find nothing either
+        m = n = 0;
+        tiles_upto = values_upto = 0;
+        return false;
+      }
+      chunk += 32;
+      load();
+    }
+    const uint32_t who = __ffs(__ballot_sync(0xFFFFFFFFu, t < tiles_before + tiles_upto)) - 1;
+    const uint64_t gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
+    const uint64_t gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
+    const uint64_t upto = __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
+    const uint64_t first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - gm * gn;
+    const uint32_t qt = static_cast<uint32_t>((gm + TQ - 1) / TQ), bt = static_cast<uint32_t>((gn + TB - 1) / TB);
+    // queries per tile: an even split, in steps of 16 (at most TQ, so that no tile is empty)
+    const uint32_t width = static_cast<uint32_t>(((gm + qt - 1) / qt + 15) / 16 * 16);
+    const uint64_t r = t - (tiles_before + upto - static_cast<uint64_t>(qt) * bt);
+    const uint32_t panel = static_cast<uint32_t>(r / (static_cast<uint64_t>(PANEL) * bt));
+    const uint64_t in_panel = r - static_cast<uint64_t>(panel) * PANEL * bt;
+    const uint32_t across = min(PANEL, qt - panel * PANEL);
+    const uint32_t bi = static_cast<uint32_t>(in_panel / across);
+    const uint32_t qi = panel * PANEL + static_cast<uint32_t>(in_panel - static_cast<uint64_t>(bi) * across);
+    const uint64_t qa = static_cast<uint64_t>(qi) * width, ba = static_cast<uint64_t>(bi) * TB;
+    out.q0 = static_cast<uint32_t>(gq + qa);
+    out.queries = static_cast<uint32_t>(min(static_cast<uint64_t>(width), gm - qa));
+    out.b0 = static_cast<uint32_t>(gb + ba);
+    out.rows = static_cast<uint32_t>(min(static_cast<uint64_t>(TB), gn - ba));
+    if (g.b_offsets) {
+      out.stride = gn;
+      out.at = first_value + qa * gn + ba;
+    } else {
+      out.stride = g.stride;
+      out.at = (gq + qa) * g.stride + ba;
+    }
+    return true;
+  }
+};
+
+}  // namespace bq
+}  // namespace pxc
