@@ -4,6 +4,8 @@
 #include <type_traits>
 
 #include "bq.cuh"
+#include "bq_tc.cuh"
+#include "tmap.cuh"
 
 namespace pxc {
 namespace bq {
@@ -67,86 +69,6 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (c0 + k < dim) dst[k] = from_f32<T>(v[k]);
-  }
-}
-
-// ---- product ----
-struct Operand {
-  const uint8_t* codes;
-  const uint8_t* scales;
-  uint64_t ld, sld;
-};
-
-// 64 queries x 64 rows per block and 16 values a thread, 32 components at a time through shared
-// memory as f32.
-constexpr uint32_t PT = 64, PK = 32;
-template <class T>
-__global__ void __launch_bounds__(256) product_kernel(Operand q, Operand b, uint32_t dim, Groups groups, T* out) {
-  __shared__ float sq[PK][PT + 4], sb[PK][PT + 4];
-  __shared__ Tile tile;
-  __shared__ uint32_t found;
-  const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  Walk<PT, PT> walk(groups, threadIdx.x & 31);
-  for (uint64_t t = blockIdx.x;; t += gridDim.x) {
-    if (threadIdx.x < 32) {
-      Tile mine;
-      const bool any = walk.find(t, mine);
-      if (threadIdx.x == 0) {
-        found = any;
-        if (any) tile = mine;
-      }
-    }
-    __syncthreads();
-    if (!found) return;
-    const Tile w = tile;
-    float acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < dim; k0 += PK) {
-      // 64 rows x 8 quads of codes on either side: two quads a thread
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t i = threadIdx.x + h * 256, row = i >> 3, c = k0 + (i & 7) * 4;
-        float2 lo = {0, 0}, hi = {0, 0};
-        if (row < w.queries && c < dim) {
-          const uint64_t r = w.q0 + row;
-          const uint32_t four = *reinterpret_cast<const uint32_t*>(q.codes + r * q.ld + c);
-          const float f = scale_value(q.scales[r * q.sld + c / BLOCK]);
-          lo = from_codes(four & 0xFFFFu), hi = from_codes(four >> 16);
-          lo.x *= f, lo.y *= f, hi.x *= f, hi.y *= f;
-        }
-        const uint32_t kk = (i & 7) * 4;
-        sq[kk][row] = lo.x, sq[kk + 1][row] = c + 1 < dim ? lo.y : 0.f;
-        sq[kk + 2][row] = c + 2 < dim ? hi.x : 0.f, sq[kk + 3][row] = c + 3 < dim ? hi.y : 0.f;
-        lo = {0, 0}, hi = {0, 0};
-        if (row < w.rows && c < dim) {
-          const uint64_t r = w.b0 + row;
-          const uint32_t four = *reinterpret_cast<const uint32_t*>(b.codes + r * b.ld + c);
-          const float f = scale_value(b.scales[r * b.sld + c / BLOCK]);
-          lo = from_codes(four & 0xFFFFu), hi = from_codes(four >> 16);
-          lo.x *= f, lo.y *= f, hi.x *= f, hi.y *= f;
-        }
-        sb[kk][row] = lo.x, sb[kk + 1][row] = c + 1 < dim ? lo.y : 0.f;
-        sb[kk + 2][row] = c + 2 < dim ? hi.x : 0.f, sb[kk + 3][row] = c + 3 < dim ? hi.y : 0.f;
-      }
-      __syncthreads();
-#pragma unroll 8
-      for (uint32_t k = 0; k < PK; ++k) {
-        float a[4], c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = sq[k][ty * 4 + i], c[i] = sb[k][tx + 16 * i];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * c[j];
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t y = ty * 4 + i, x = tx + 16 * j;
-        if (y < w.queries && x < w.rows) out[w.at + y * w.stride + x] = from_f32<T>(acc[i][j]);
-      }
   }
 }
 
@@ -228,16 +150,44 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
   count_launch(ctx);
 }
 
-static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, Groups g, void* out,
+static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, const Groups& g, void* out,
                     int32_t dtype, cudaStream_t s) {
-  g.nq = q.rows;
-  g.nb = b.rows;
-  g.faults = ctx->bq_faults;
+  using namespace bq_tc;
+  Params p{};
+  p.groups = g;
+  p.groups.nq = q.rows;
+  p.groups.nb = b.rows;
+  p.groups.faults = ctx->bq_faults;
+  p.q_scales = q.scales;
+  p.b_scales = b.scales;
+  p.q_sld = q.sld;
+  p.b_sld = b.sld;
+  p.out = out;
+  p.dim = dim;
+  p.kblocks = blocks_of(dim);
+  uint64_t tiles;
+  if (!g.q_offsets) {
+    // the walk's even split: every tile but the last is this wide, one box brings it
+    const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
+    p.q_rows = p.q_box = static_cast<uint32_t>(up((q.rows + qt - 1) / qt, 16));
+    tiles = qt * ((b.rows + BM - 1) / BM);
+  } else {
+    // groups of any size: room for the widest tile, filled by as many boxes as a tile needs
+    p.q_box = 32;
+    p.q_rows = static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, up(q.rows, 32)));
+    tiles = g.b_offsets ? ctx->sm_count : (g.groups + q.rows / MAX_Q) * ((g.n_each + BM - 1) / BM);
+  }
+  p.stages = pick_stages(p.q_rows);
+  p.wait_ns = static_cast<uint64_t>(ctx->wait_ms) * 1000000ull;
+  CUtensorMap map_b, map_q;
+  make_tmap_u8_pitched(&map_b, b.codes, dim, b.ld, b.rows, BM);
+  make_tmap_u8_pitched(&map_q, q.codes, dim, q.ld, q.rows, p.q_box);
+  const uint32_t smem = smem_bytes(p.q_rows, p.stages);
+  const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(tiles, 1)));
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    product_kernel<T><<<ctx->sm_count * 4, 256, 0, s>>>(Operand{q.codes, q.scales, q.ld, q.sld},
-                                                        Operand{b.codes, b.scales, b.ld, b.sld}, dim, g,
-                                                        static_cast<T*>(out));
+    PXC_CUDA(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    product_kernel<T><<<grid, THREADS, smem, s>>>(map_b, map_q, p);
   });
   PXC_CUDA(cudaGetLastError());
   count_launch(ctx);
