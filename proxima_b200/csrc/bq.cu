@@ -177,12 +177,11 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
     p.q_rows = static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, up(q.rows, 32)));
     tiles = g.b_offsets ? ctx->sm_count : (g.groups + q.rows / MAX_Q) * ((g.n_each + BM - 1) / BM);
   }
-  p.stages = pick_stages(p.q_rows);
-  p.wait_ns = static_cast<uint64_t>(ctx->wait_ms) * 1000000ull;
+  p.wait_cycles = static_cast<uint64_t>(ctx->wait_ms) * 2000000ull;  // the SM clock is below 2 GHz
   CUtensorMap map_b, map_q;
   make_tmap_u8_pitched(&map_b, b.codes, dim, b.ld, b.rows, BM);
   make_tmap_u8_pitched(&map_q, q.codes, dim, q.ld, q.rows, p.q_box);
-  const uint32_t smem = smem_bytes(p.q_rows, p.stages);
+  const uint32_t smem = plan(p);
   const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(tiles, 1)));
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;

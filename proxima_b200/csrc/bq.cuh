@@ -99,21 +99,26 @@ struct Tile {
 
 // Walks the tiles in order, a warp at a time: lane i holds group chunk + i. Tiles are numbered
 // through the groups; find() is called with rising numbers, so that each chunk of 32 groups is
-// read once. Inside a group the queries come in panels of PANEL tiles, so that a panel's
-// queries stay in L2 while the base rows pass once.
+// read once. Inside a group the base rows come in panels of PANEL tiles, all queries against
+// one panel before the next: neighbouring CTAs write neighbouring columns of the same
+// output rows, and a panel's rows stay in L2 while the queries pass.
 //
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
 // matrix ends within the output. One that fails counts as empty and leaves a fault, so
 // that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
 template <uint32_t TQ, uint32_t TB>
 struct Walk {
-  static constexpr uint32_t PANEL = 16;
+  static constexpr uint32_t PANEL = 64;
   const Groups& g;
   const uint32_t lane;
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
   uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
   uint64_t q0 = 0, b0 = 0, m = 0, n = 0;
+  // the group found last, in every lane: its tiles are [first, last)
+  uint64_t first = 0, last = 0;
+  uint64_t gq = 0, gb = 0, gm = 0, gn = 0, first_value = 0;
+  uint32_t qt = 0, bt = 0, width = 0;
 
   __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id) : g(groups), lane(lane_id) { load(); }
 
@@ -170,6 +175,45 @@ struct Walk {
 
   // Tile number t, or false when there are fewer. All lanes call and get the same answer.
   __device__ __forceinline__ bool find(uint64_t t, Tile& out) {
+    if (t >= last && !enter(t)) return false;
+    const uint64_t r = t - first;
+    uint32_t qi, bi;
+    if (last - first <= 0xFFFFFFFFu) {
+      const uint32_t r32 = static_cast<uint32_t>(r);
+      if (qt == 1) {
+        qi = 0, bi = r32;
+      } else {
+        // at most 2^32 / bt tiles of queries, so a panel's PANEL * qt tiles fit 32 bits whenever bt >= PANEL
+        const uint32_t panel = bt <= PANEL ? 0 : r32 / (PANEL * qt);
+        const uint32_t in_panel = r32 - panel * PANEL * qt;
+        const uint32_t across = min(PANEL, bt - panel * PANEL);
+        qi = in_panel / across;
+        bi = panel * PANEL + in_panel - qi * across;
+      }
+    } else {
+      const uint32_t panel = static_cast<uint32_t>(r / (static_cast<uint64_t>(PANEL) * qt));
+      const uint64_t in_panel = r - static_cast<uint64_t>(panel) * PANEL * qt;
+      const uint32_t across = min(PANEL, bt - panel * PANEL);
+      qi = static_cast<uint32_t>(in_panel / across);
+      bi = panel * PANEL + static_cast<uint32_t>(in_panel - static_cast<uint64_t>(qi) * across);
+    }
+    const uint64_t qa = static_cast<uint64_t>(qi) * width, ba = static_cast<uint64_t>(bi) * TB;
+    out.q0 = static_cast<uint32_t>(gq + qa);
+    out.queries = static_cast<uint32_t>(min(static_cast<uint64_t>(width), gm - qa));
+    out.b0 = static_cast<uint32_t>(gb + ba);
+    out.rows = static_cast<uint32_t>(min(static_cast<uint64_t>(TB), gn - ba));
+    if (g.b_offsets) {
+      out.stride = gn;
+      out.at = first_value + qa * gn + ba;
+    } else {
+      out.stride = g.stride;
+      out.at = (gq + qa) * g.stride + ba;
+    }
+    return true;
+  }
+
+  // Goes on to the group that holds tile t.
+  __device__ __forceinline__ bool enter(uint64_t t) {
     for (;;) {
       const uint64_t total = __shfl_sync(0xFFFFFFFFu, tiles_upto, 31);
       if (t < tiles_before + total) break;
@@ -185,31 +229,14 @@ struct Walk {
       load();
     }
     const uint32_t who = __ffs(__ballot_sync(0xFFFFFFFFu, t < tiles_before + tiles_upto)) - 1;
-    const uint64_t gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
-    const uint64_t gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
-    const uint64_t upto = __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
-    const uint64_t first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - gm * gn;
-    const uint32_t qt = static_cast<uint32_t>((gm + TQ - 1) / TQ), bt = static_cast<uint32_t>((gn + TB - 1) / TB);
+    gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
+    gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
+    first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - gm * gn;
+    qt = static_cast<uint32_t>((gm + TQ - 1) / TQ), bt = static_cast<uint32_t>((gn + TB - 1) / TB);
     // queries per tile: an even split, in steps of 16 (at most TQ, so that no tile is empty)
-    const uint32_t width = static_cast<uint32_t>(((gm + qt - 1) / qt + 15) / 16 * 16);
-    const uint64_t r = t - (tiles_before + upto - static_cast<uint64_t>(qt) * bt);
-    const uint32_t panel = static_cast<uint32_t>(r / (static_cast<uint64_t>(PANEL) * bt));
-    const uint64_t in_panel = r - static_cast<uint64_t>(panel) * PANEL * bt;
-    const uint32_t across = min(PANEL, qt - panel * PANEL);
-    const uint32_t bi = static_cast<uint32_t>(in_panel / across);
-    const uint32_t qi = panel * PANEL + static_cast<uint32_t>(in_panel - static_cast<uint64_t>(bi) * across);
-    const uint64_t qa = static_cast<uint64_t>(qi) * width, ba = static_cast<uint64_t>(bi) * TB;
-    out.q0 = static_cast<uint32_t>(gq + qa);
-    out.queries = static_cast<uint32_t>(min(static_cast<uint64_t>(width), gm - qa));
-    out.b0 = static_cast<uint32_t>(gb + ba);
-    out.rows = static_cast<uint32_t>(min(static_cast<uint64_t>(TB), gn - ba));
-    if (g.b_offsets) {
-      out.stride = gn;
-      out.at = first_value + qa * gn + ba;
-    } else {
-      out.stride = g.stride;
-      out.at = (gq + qa) * g.stride + ba;
-    }
+    width = static_cast<uint32_t>(((gm + qt - 1) / qt + 15) / 16 * 16);
+    last = tiles_before + __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
+    first = last - static_cast<uint64_t>(qt) * bt;
     return true;
   }
 };
