@@ -181,6 +181,18 @@ struct Reader {
   }
 };
 
+// One lane of a converged warp, in a form from which the compiler knows that it is one: the operands of
+// the tensor instructions then need no loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 __device__ __forceinline__ uint32_t round16(uint32_t x) { return (x + 15) & ~15u; }
 
 template <class T>
@@ -225,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     // ---- producer ----
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t issued = 0, s = 0, ph = 0;
       bool ok = true;
       while (ok && reader.next_one(t)) {
@@ -251,7 +263,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     // ---- MMA ----
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t s = 0, ph = 0;                // stage ring
       uint32_t quad = 0, sf = 0, sf_ph = 0;  // scale words: number, slot
       uint32_t acc = 0, acc_ph = 0;
