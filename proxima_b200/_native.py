@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from pathlib import Path
 
 from .errors import raise_for_status
@@ -309,6 +310,29 @@ def call(name: str, *args) -> None:
     if status != 0:
         raise_for_status(status, err.a, err.b, err.parameter.decode(errors="replace"),
                          err.detail.decode(errors="replace"))
+
+
+_errors = threading.local()
+
+
+def bind(name: str):
+    """``call`` for one entry point that is called often: its function and each thread's error struct
+    (cleared by every successful call) are looked up once."""
+    fn = getattr(load(), name)
+
+    def bound(*args) -> None:
+        try:
+            err, ref = _errors.pair
+        except AttributeError:
+            err = PxcError()
+            ref = C.byref(err)
+            _errors.pair = err, ref
+        status = fn(*args, ref)
+        if status != 0:
+            raise_for_status(status, err.a, err.b, err.parameter.decode(errors="replace"),
+                             err.detail.decode(errors="replace"))
+
+    return bound
 
 
 def ptr(arr) -> int | None:

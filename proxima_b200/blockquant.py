@@ -29,11 +29,12 @@ from . import _native as N
 from .errors import Configuration, DimensionMismatch
 
 BLOCK = 128
-_DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_NAMES = {"float32": 0, "float16": 1, "bfloat16": 2}
+_codes: dict = {}  # dtype -> its code, torch's types among them once torch is in use
 
 
 def _is_cuda(x) -> bool:
-    return hasattr(x, "is_cuda") and x.is_cuda
+    return getattr(x, "is_cuda", False)
 
 
 def _up(x: int, to: int) -> int:
@@ -41,10 +42,36 @@ def _up(x: int, to: int) -> int:
 
 
 def _dtype_code(dtype) -> int:
-    name = str(dtype).split(".")[-1] if "torch" in str(dtype) else np.dtype(dtype).name
-    if name not in _DTYPES:
-        raise Configuration("dtype", 0, f"{name}: must be float32, float16 or bfloat16 (tensors only)")
-    return _DTYPES[name]
+    code = _codes.get(dtype)
+    if code is None:
+        name = str(dtype).split(".")[-1] if "torch" in str(dtype) else np.dtype(dtype).name
+        if name not in _NAMES:
+            raise Configuration("dtype", 0, f"{name}: must be float32, float16 or bfloat16 (tensors only)")
+        code = _codes[dtype] = _NAMES[name]
+    return code
+
+
+class _Torch:
+    """What the tensor paths take from torch, and their entry points, looked up once."""
+
+    def __init__(self):
+        import torch
+
+        self.uint8, self.int64, self.float32, self.empty = torch.uint8, torch.int64, torch.float32, torch.empty
+        self.current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        self.encode, self.decode = N.bind("pxc_bq_encode_device"), N.bind("pxc_bq_decode_device")
+        self.product, self.grouped = N.bind("pxc_bq_product_device"), N.bind("pxc_bq_grouped_product_device")
+
+
+_torch_parts: _Torch | None = None
+
+
+def _torch() -> _Torch:
+    global _torch_parts
+    if _torch_parts is None:
+        _torch_parts = _Torch()
+    return _torch_parts
 
 
 @dataclass
@@ -80,33 +107,45 @@ class BlockQuantizer:
         self.dim = int(dim)
         self.blocks = -(-self.dim // BLOCK)
         self.ctx = context or Context.default()
+        self._ld, self._sld = _up(self.dim, 16), _up(self.blocks, 4)
 
     # -- arguments --
     def _stream(self, tensor) -> int:
         """The current stream of the tensor's device; 1 names the legacy default stream."""
-        import torch
-
-        if tensor.device.index != self.ctx.device:
-            raise Configuration("device", tensor.device.index, f"the context is on device {self.ctx.device}")
-        return torch.cuda.current_stream(tensor.device).cuda_stream or 1
+        index = tensor.get_device()
+        if index != self.ctx.device:
+            raise Configuration("device", index, f"the context is on device {self.ctx.device}")
+        return _torch().current_stream(index) or 1
 
     def _rows(self, c: BlockCodes, cuda: bool, name: str, device=None) -> N.PxcBqRows:
         if c.dim != self.dim:
             raise DimensionMismatch(self.dim, c.dim)
-        out = []
-        for a, unit, need in ((c.codes, 16, _up(self.dim, 16)), (c.scales, 4, _up(self.blocks, 4))):
-            if _is_cuda(a) != cuda or (cuda and device is not None and a.device != device):
+        codes, scales = c.codes, c.scales
+        if cuda:
+            if not (_is_cuda(codes) and _is_cuda(scales)) or codes.device != scales.device or (
+                    device is not None and codes.device != device):
                 raise Configuration(name, 0, "all operands on one device, or all on the host")
-            if str(a.dtype).split(".")[-1] != "uint8" or a.ndim != 2 or a.shape[0] != len(c) or a.shape[1] < need:
-                raise Configuration(name, 0, f"codes and scales are uint8, (n, >= {need}) here")
-            row, step = (a.stride(0), a.stride(1)) if cuda else a.strides
-            if step != 1 or (a.shape[0] > 1 and (row % unit or row < need)):
-                raise Configuration(name, 0, f"rows are contiguous, their pitch a multiple of {unit}")
-            out.append(row if a.shape[0] > 1 else need)
-        return N.PxcBqRows(N.ptr(c.codes), N.ptr(c.scales), len(c), out[0], out[1])
+            byte = _torch().uint8
+            (cr, cs), (sr, ss) = codes.stride() if codes.ndim == 2 else (0, 0), scales.stride() if scales.ndim == 2 else (0, 0)
+        else:
+            if _is_cuda(codes) or _is_cuda(scales):
+                raise Configuration(name, 0, "all operands on one device, or all on the host")
+            byte = np.uint8
+            (cr, cs), (sr, ss) = codes.strides if codes.ndim == 2 else (0, 0), scales.strides if scales.ndim == 2 else (0, 0)
+        if codes.dtype != byte or scales.dtype != byte or codes.ndim != 2 or scales.ndim != 2:
+            raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
+        n, width = codes.shape
+        rows, blocks = scales.shape
+        if rows != n or width < self._ld or blocks < self._sld:
+            raise Configuration(name, n, f"codes are (n, >= {self._ld}) and scales (n, >= {self._sld}) here")
+        if n <= 1:
+            cr, sr = self._ld, self._sld
+        if cs != 1 or ss != 1 or cr % 16 or sr % 4 or cr < self._ld or sr < self._sld:
+            raise Configuration(name, n, "rows are contiguous, the codes' pitch a multiple of 16, the scales' of 4")
+        return N.PxcBqRows(N.ptr(codes), N.ptr(scales), n, cr, sr)
 
     def _vectors(self, vectors):
-        """(n, dim) with contiguous components, in one of the types."""
+        """(n, dim), an array in one of the types."""
         if _is_cuda(vectors):
             v = vectors
         else:
@@ -124,19 +163,19 @@ class BlockQuantizer:
         """Each row's codes and scales. Rows of a tensor may be strided. An infinity becomes the
         largest code of its block, 448 times the scale; a NaN stays one."""
         v = self._vectors(vectors)
-        n, ld, sld = v.shape[0], _up(self.dim, 16), _up(self.blocks, 4)
+        n, ld, sld = v.shape[0], self._ld, self._sld
         if _is_cuda(v):
-            import torch
-
+            t = _torch()
             code = _dtype_code(v.dtype)
             stream = self._stream(v)
-            if (self.dim > 1 and v.stride(1) != 1) or (n > 1 and v.stride(0) < self.dim):
+            row, step = v.stride()
+            if (self.dim > 1 and step != 1) or (n > 1 and row < self.dim):
                 v = v.contiguous()
-            codes = torch.empty((n, ld), dtype=torch.uint8, device=v.device)
-            scales = torch.empty((n, sld), dtype=torch.uint8, device=v.device)
+                row = self.dim
+            codes = t.empty((n, ld), dtype=t.uint8, device=v.device)
+            scales = t.empty((n, sld), dtype=t.uint8, device=v.device)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
-            N.call("pxc_bq_encode_device", self.ctx.handle, v.data_ptr(), code, v.stride(0) if n > 1 else self.dim,
-                   self.dim, C.byref(rows), stream)
+            t.encode(self.ctx.handle, v.data_ptr(), code, row if n > 1 else self.dim, self.dim, C.byref(rows), stream)
             return BlockCodes(codes, scales, self.dim)
         v = np.ascontiguousarray(v)
         codes, scales = np.zeros((n, ld), np.uint8), np.zeros((n, sld), np.uint8)
@@ -149,11 +188,10 @@ class BlockQuantizer:
         cuda = _is_cuda(codes.codes)
         rows = self._rows(codes, cuda, "codes")
         if cuda:
-            import torch
-
-            out = torch.empty((len(codes), self.dim), dtype=dtype or torch.float32, device=codes.codes.device)
-            N.call("pxc_bq_decode_device", self.ctx.handle, C.byref(rows), self.dim, out.data_ptr(),
-                   _dtype_code(out.dtype), self.dim, self._stream(out))
+            t = _torch()
+            code = _dtype_code(dtype or t.float32)
+            out = t.empty((rows.rows, self.dim), dtype=dtype or t.float32, device=codes.codes.device)
+            t.decode(self.ctx.handle, C.byref(rows), self.dim, out.data_ptr(), code, self.dim, self._stream(out))
             return out
         out = np.zeros((len(codes), self.dim), dtype or np.float32)
         N.call("pxc_bq_decode", self.ctx.handle, C.byref(rows), self.dim, N.ptr(out), _dtype_code(out.dtype), self.dim)
@@ -164,19 +202,22 @@ class BlockQuantizer:
         """The dot product of every pair of rows, (nq, n): f32 sums, rounded once to ``dtype``
         (float32). ``out`` may be a tensor to write into, its rows strided."""
         cuda = _is_cuda(queries.codes)
-        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base", queries.codes.device if cuda else None)
-        shape = (len(queries), len(base))
+        dev = queries.codes.device if cuda else None
+        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base", dev)
+        shape = (q.rows, b.rows)
         if cuda:
-            import torch
-
-            dev = queries.codes.device
+            t = _torch()
+            stride = shape[1] or 1
             if out is None:
-                out = torch.empty(shape, dtype=dtype or torch.float32, device=dev)
-            elif (tuple(out.shape) != shape or out.device != dev or (dtype is not None and out.dtype != dtype)
-                  or (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1])):
-                raise Configuration("out", 0, "must be (nq, n) on the operands' device, with contiguous rows")
-            N.call("pxc_bq_product_device", self.ctx.handle, C.byref(q), C.byref(b), self.dim, out.data_ptr(),
-                   _dtype_code(out.dtype), out.stride(0) if shape[0] > 1 else max(shape[1], 1), self._stream(out))
+                code = _dtype_code(dtype or t.float32)
+                out = t.empty(shape, dtype=dtype or t.float32, device=dev)
+            else:
+                if (tuple(out.shape) != shape or out.device != dev or (dtype is not None and out.dtype != dtype)
+                        or (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1])):
+                    raise Configuration("out", 0, "must be (nq, n) on the operands' device, with contiguous rows")
+                code = _dtype_code(out.dtype)
+                stride = out.stride(0) if shape[0] > 1 else stride
+            t.product(self.ctx.handle, C.byref(q), C.byref(b), self.dim, out.data_ptr(), code, stride, self._stream(out))
             return out
         if out is not None:
             raise Configuration("out", 0, "is for tensors")
@@ -202,22 +243,23 @@ class BlockQuantizer:
             raise Configuration("offsets", 0, "groups + 1 int64 values for the queries, and for the base where given")
         groups = len(qo) - 1
         if bo is None:
-            if len(base) % groups:
-                raise Configuration("base", len(base), "without base offsets the rows must be a multiple of the groups")
-            shape = (len(queries), len(base) // groups)
+            if b.rows % groups:
+                raise Configuration("base", b.rows, "without base offsets the rows must be a multiple of the groups")
+            shape = (q.rows, b.rows // groups)
+            size = shape[0] * shape[1]
         else:
             if out_size is None:
                 out_size = int(((qo[1:] - qo[:-1]) * (bo[1:] - bo[:-1])).sum())
-                if out_size < 0:
-                    raise Configuration("offsets", 0, "offsets must rise")
-            shape = (int(out_size),)
-        size = int(np.prod(shape, dtype=np.int64))
+            if out_size < 0:
+                raise Configuration("offsets", 0, "offsets must rise")
+            size = int(out_size)
+            shape = (size,)
         if cuda:
-            import torch
-
-            out = torch.empty(shape, dtype=dtype or torch.float32, device=dev)
-            N.call("pxc_bq_grouped_product_device", self.ctx.handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo),
-                   groups, self.dim, out.data_ptr(), _dtype_code(out.dtype), size, self._stream(out))
+            t = _torch()
+            code = _dtype_code(dtype or t.float32)
+            out = t.empty(shape, dtype=dtype or t.float32, device=dev)
+            t.grouped(self.ctx.handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups, self.dim, out.data_ptr(),
+                      code, size, self._stream(out))
             return out
         out = np.zeros(shape, dtype or np.float32)
         N.call("pxc_bq_grouped_product", self.ctx.handle, C.byref(q), N.ptr(qo), C.byref(b), N.ptr(bo), groups, self.dim,
@@ -228,14 +270,11 @@ class BlockQuantizer:
         if o is None:
             return None
         if cuda:
-            if not _is_cuda(o) or o.device != dev or str(o.dtype) != "torch.int64" or o.ndim != 1:
+            if not _is_cuda(o) or o.device != dev or o.dtype != _torch().int64 or o.ndim != 1:
                 raise Configuration("offsets", 0, "must be an int64 tensor on the operands' device")
             return o.contiguous()
         return np.ascontiguousarray(o, np.int64)
 
     def check(self) -> None:
         """Waits for the current stream and raises a failure that an earlier call left on the device."""
-        import torch
-
-        stream = torch.cuda.current_stream(self.ctx.device).cuda_stream or 1
-        N.call("pxc_bq_check", self.ctx.handle, stream)
+        N.call("pxc_bq_check", self.ctx.handle, _torch().current_stream(self.ctx.device) or 1)

@@ -185,7 +185,10 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(tiles, 1)));
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    PXC_CUDA(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    if (!(__atomic_load_n(&ctx->bq_ready, __ATOMIC_ACQUIRE) & (1u << dtype))) {  // once per context and type
+      PXC_CUDA(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+      __atomic_fetch_or(&ctx->bq_ready, 1u << dtype, __ATOMIC_RELEASE);
+    }
     product_kernel<T><<<grid, THREADS, smem, s>>>(map_b, map_q, p);
   });
   PXC_CUDA(cudaGetLastError());
