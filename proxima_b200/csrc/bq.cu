@@ -17,58 +17,314 @@ constexpr uint64_t MAX_SIZE = uint64_t(1) << 48;  // values in an output: offset
 static uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 static uint32_t blocks_of(uint32_t dim) { return (dim + BLOCK - 1) / BLOCK; }
 
-// ---- encode ----
-// A warp per block of 128: four components a lane, the largest magnitude by one warp reduction,
-// one packed store of the four codes.
+// ---- encode and decode ----
+// Both should be bound by the bytes they read and write, which leaves some 25 instructions of a warp per
+// block of 128. So eight lanes share a block and a warp works on four rows at once: a lane
+// moves 16 bytes of vector at a time, and what is done once per block (the reduction, the scale, the
+// addresses) is done for four. Items go by a fixed step: no division stands in the loop.
+//
+// Where rows do not start on 16 bytes (an odd pitch or base), a whole warp takes a block, its lanes single
+// components 32 apart: each access covers neighbouring bytes, and whole sectors of the codes.
+
+// The items of one warp: a block of the R rows from `row` on.
+template <uint32_t R>
+struct Items {
+  uint64_t row;
+  uint32_t block;
+  __device__ __forceinline__ Items(uint32_t blocks) {
+    const uint32_t number = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    row = static_cast<uint64_t>(number / blocks) * R;
+    block = number % blocks;
+  }
+  __device__ __forceinline__ void next(uint64_t step_rows, uint32_t step_blocks, uint32_t blocks) {
+    row += step_rows;
+    if (step_blocks == 0) {
+      // a step of whole rows would leave a warp at one block of them, the short last one always to the
+      // same warps: all of a step's items move on by one block together
+      block = block + 1 == blocks ? 0 : block + 1;
+    } else {
+      block += step_blocks;
+      if (block >= blocks) block -= blocks, row += R;
+    }
+  }
+};
+
+template <class T>
+constexpr uint32_t CHUNK = 16 / sizeof(T);  // components in 16 bytes
+template <class T>
+constexpr uint32_t WIDE_ROWS = sizeof(T) == 4 ? 4 : 8;  // 2 KB of vectors per warp in flight either way
+constexpr uint32_t NARROW_ROWS = 4;
+
+// 16 bytes of components as f32, and back.
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& q, float (&v)[CHUNK<T>]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, float>) {
+      v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 pack(const float (&v)[CHUNK<T>]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, float>) {
+      w[i] = __float_as_uint(v[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One row's scale byte, and the padding behind the last.
+__device__ __forceinline__ void store_scale(uint8_t* row, uint32_t block, uint32_t blocks, uint32_t byte) {
+  if (blocks == 1) {
+    *reinterpret_cast<uint32_t*>(row) = byte;
+  } else {
+    row[block] = static_cast<uint8_t>(byte);
+    if (block + 1 == blocks)
+      for (uint32_t k = blocks; k & 3; ++k) row[k] = 0;
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(256)
-    encode_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
-                  uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld) {
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t warps = static_cast<uint64_t>(gridDim.x) * (blockDim.x >> 5);
-  const uint64_t total = rows * blocks;
+    encode_wide_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
+                       uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld,
+                       uint64_t step_rows, uint32_t step_blocks) {
+  constexpr uint32_t V = CHUNK<T>, C = 16 / V, R = WIDE_ROWS<T>, U = R / 4;
+  const uint32_t lane = threadIdx.x & 31, l = lane & 7, group = lane >> 3;
   const uint32_t code_end = (dim + 15) / 16 * 16;
-  for (uint64_t w = static_cast<uint64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps) {
-    const uint64_t r = w / blocks;
-    const uint32_t j = static_cast<uint32_t>(w - r * blocks);
-    const uint32_t c0 = j * BLOCK + lane * 4;
-    const T* row = x + r * stride;
-    float v[4];
+  for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
+    const uint32_t c0 = it.block * BLOCK + l * V;  // chunk k: 8 * V further each
+    float v[U][C][V];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c0 + i < dim ? to_f32<T>(row[c0 + i]) : 0.0f;
-    const uint32_t top = max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
-    const uint32_t byte = scale_byte(__reduce_max_sync(0xFFFFFFFFu, top));
-    const float f = inverse_scale(byte);
-    if (c0 < code_end)
-      *reinterpret_cast<uint32_t*>(codes + r * ld + c0) = to_codes(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
-    if (lane == 0) {
-      uint8_t* s = scales + r * sld;
-      s[j] = static_cast<uint8_t>(byte);
-      if (j + 1 == blocks)
-        for (uint32_t k = blocks; k & 3; ++k) s[k] = 0;
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint64_t r = it.row + u * 4 + group;
+      const T* p = x + r * stride + c0;
+#pragma unroll
+      for (uint32_t k = 0; k < C; ++k) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (r < rows && c0 + k * 8 * V + V <= dim) q = __ldcs(reinterpret_cast<const uint4*>(p + k * 8 * V));
+        unpack<T>(q, v[u][k]);
+      }
+    }
+    if (dim % V != 0 && it.block + 1 == blocks) {  // the components behind the last whole chunk
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint64_t r = it.row + u * 4 + group;
+#pragma unroll
+        for (uint32_t k = 0; k < C; ++k) {
+          const uint32_t c = c0 + k * 8 * V;
+          if (r < rows && c < dim && c + V > dim)
+#pragma unroll
+            for (uint32_t i = 0; i < V - 1; ++i)
+              if (c + i < dim) v[u][k][i] = to_f32<T>(x[r * stride + c + i]);
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      // fmax passes over NaN; an infinity is left out when it shows
+      float top = 0.0f;
+#pragma unroll
+      for (uint32_t k = 0; k < C; ++k)
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) top = fmaxf(top, fabsf(v[u][k][i]));
+#pragma unroll
+      for (uint32_t d = 4; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+      if (__any_sync(0xFFFFFFFFu, __float_as_uint(top) == 0x7F800000u)) {
+        uint32_t finite = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < C; ++k)
+#pragma unroll
+          for (uint32_t i = 0; i < V; ++i) finite = max(finite, finite_bits(v[u][k][i]));
+#pragma unroll
+        for (uint32_t d = 4; d; d >>= 1) finite = max(finite, __shfl_xor_sync(0xFFFFFFFFu, finite, d));
+        top = __uint_as_float(finite);
+      }
+      const uint32_t byte = scale_byte(__float_as_uint(top));
+      const float f = inverse_scale(byte);
+      const uint64_t r = it.row + u * 4 + group;
+      if (r < rows) {
+        uint8_t* to = codes + r * ld + c0;
+#pragma unroll
+        for (uint32_t k = 0; k < C; ++k) {
+          uint32_t four[V / 4];
+#pragma unroll
+          for (uint32_t i = 0; i < V; i += 4)
+            four[i / 4] = to_codes(v[u][k][i] * f, v[u][k][i + 1] * f, v[u][k][i + 2] * f, v[u][k][i + 3] * f);
+          if (c0 + k * 8 * V < code_end) {
+            if constexpr (V == 4)
+              *reinterpret_cast<uint32_t*>(to + k * 32) = four[0];
+            else
+              *reinterpret_cast<uint2*>(to + k * 64) = make_uint2(four[0], four[1]);
+          }
+        }
+        if (l == 0) store_scale(scales + r * sld, it.block, blocks, byte);
+      }
     }
   }
 }
 
-// ---- decode ----
+// One item; WHOLE: all rows and the whole block are there, so nothing is tested.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void encode_narrow(const T* __restrict__ p, uint64_t stride, uint32_t n, uint32_t left,
+                                              uint32_t code_left, uint8_t* __restrict__ to, uint64_t ld,
+                                              uint8_t* __restrict__ s, uint64_t sld, uint32_t block, uint32_t blocks,
+                                              uint32_t lane) {
+  constexpr uint32_t R = NARROW_ROWS;
+  float v[R][4];
+#pragma unroll
+  for (uint32_t u = 0; u < R; ++u, p += stride)
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) v[u][k] = WHOLE || (u < n && 32 * k < left) ? to_f32<T>(p[32 * k]) : 0.0f;
+#pragma unroll
+  for (uint32_t u = 0; u < R; ++u, to += ld, s += sld) {
+    const float most = fmaxf(fmaxf(fabsf(v[u][0]), fabsf(v[u][1])), fmaxf(fabsf(v[u][2]), fabsf(v[u][3])));
+    uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
+    if (top >= 0x7F800000u)
+      top = __reduce_max_sync(0xFFFFFFFFu, max(max(finite_bits(v[u][0]), finite_bits(v[u][1])),
+                                               max(finite_bits(v[u][2]), finite_bits(v[u][3]))));
+    const uint32_t byte = scale_byte(top);
+    const float f = inverse_scale(byte);
+    const uint32_t four = to_codes(v[u][0] * f, v[u][1] * f, v[u][2] * f, v[u][3] * f);
+    if (WHOLE || u < n) {
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        if (WHOLE || 32 * k < code_left) to[32 * k] = static_cast<uint8_t>(four >> (8 * k));
+      if (lane == 0) store_scale(s, block, blocks, byte);
+    }
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(256)
-    decode_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales, uint64_t sld,
-                  uint64_t rows, uint32_t dim, T* __restrict__ out, uint64_t stride) {
-  const uint32_t quads = (dim + 3) / 4;
-  const uint64_t total = rows * quads;
-  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
-    const uint64_t r = i / quads;
-    const uint32_t c0 = static_cast<uint32_t>(i - r * quads) * 4;
-    const uint32_t four = *reinterpret_cast<const uint32_t*>(codes + r * ld + c0);
-    const float f = scale_value(scales[r * sld + c0 / BLOCK]);
-    const float2 a = from_codes(four & 0xFFFFu), b = from_codes(four >> 16);
-    const float v[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
-    T* dst = out + r * stride + c0;
+    encode_narrow_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
+                         uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld,
+                         uint64_t step_rows, uint32_t step_blocks) {
+  constexpr uint32_t R = NARROW_ROWS;
+  const uint32_t lane = threadIdx.x & 31, code_end = (dim + 15) / 16 * 16;
+  for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
+    const uint32_t b0 = it.block * BLOCK, c0 = b0 + lane;  // components c0 + 32 k
+    const uint32_t n = static_cast<uint32_t>(min(static_cast<uint64_t>(R), rows - it.row));
+    const T* p = x + it.row * stride + c0;
+    uint8_t* to = codes + it.row * ld + c0;
+    uint8_t* s = scales + it.row * sld;
+    if (n == R && b0 + BLOCK <= dim)
+      encode_narrow<T, true>(p, stride, R, 0, 0, to, ld, s, sld, it.block, blocks, lane);
+    else
+      encode_narrow<T, false>(p, stride, n, c0 < dim ? dim - c0 : 0, c0 < code_end ? code_end - c0 : 0, to, ld, s, sld,
+                              it.block, blocks, lane);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    decode_wide_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales, uint64_t sld,
+                       uint64_t rows, uint32_t dim, uint32_t blocks, T* __restrict__ out, uint64_t stride,
+                       uint64_t step_rows, uint32_t step_blocks) {
+  constexpr uint32_t V = CHUNK<T>, C = 16 / V, R = WIDE_ROWS<T>, U = R / 4;
+  const uint32_t lane = threadIdx.x & 31, l = lane & 7, group = lane >> 3;
+  for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
+    const uint32_t c0 = it.block * BLOCK + l * V;
+    uint32_t q[U][C][V / 4], byte[U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (c0 + k < dim) dst[k] = from_f32<T>(v[k]);
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint64_t r = it.row + u * 4 + group;
+      const uint8_t* p = codes + r * ld + c0;
+      byte[u] = r < rows ? scales[r * sld + it.block] : 0u;
+#pragma unroll
+      for (uint32_t k = 0; k < C; ++k) {
+        const bool any = r < rows && c0 + k * 8 * V < dim;  // a chunk is 4 or 8 bytes of the pitch's 16
+        if constexpr (V == 4) {
+          q[u][k][0] = any ? __ldcs(reinterpret_cast<const uint32_t*>(p + k * 32)) : 0u;
+        } else {
+          const uint2 w = any ? __ldcs(reinterpret_cast<const uint2*>(p + k * 64)) : make_uint2(0, 0);
+          q[u][k][0] = w.x, q[u][k][1] = w.y;
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint64_t r = it.row + u * 4 + group;
+      const float f = scale_value(byte[u]);
+      T* p = out + r * stride + c0;
+#pragma unroll
+      for (uint32_t k = 0; k < C; ++k) {
+        float v[V];
+#pragma unroll
+        for (uint32_t i = 0; i < V; i += 2) {
+          const float2 two = from_codes((q[u][k][i / 4] >> (8 * (i & 2))) & 0xFFFFu);
+          v[i] = two.x * f, v[i + 1] = two.y * f;
+        }
+        const uint32_t c = c0 + k * 8 * V;
+        if (r < rows && c + V <= dim) {
+          __stcs(reinterpret_cast<uint4*>(p + k * 8 * V), pack<T>(v));
+        } else if (r < rows && c < dim) {
+#pragma unroll
+          for (uint32_t i = 0; i < V - 1; ++i)
+            if (c + i < dim) p[k * 8 * V + i] = from_f32<T>(v[i]);
+        }
+      }
+    }
+  }
+}
+
+template <class T, bool WHOLE>
+__device__ __forceinline__ void decode_narrow(const uint8_t* __restrict__ p, uint64_t ld, const uint8_t* __restrict__ s,
+                                              uint64_t sld, uint32_t n, uint32_t left, T* __restrict__ to,
+                                              uint64_t stride) {
+  constexpr uint32_t R = NARROW_ROWS;
+  uint32_t code[R][4], byte[R];
+#pragma unroll
+  for (uint32_t u = 0; u < R; ++u, p += ld, s += sld) {
+    byte[u] = WHOLE || u < n ? *s : 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) code[u][k] = WHOLE || (u < n && 32 * k < left) ? p[32 * k] : 0u;
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < R; ++u, to += stride) {
+    const float f = scale_value(byte[u]);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k += 2) {
+      const float2 two = from_codes(code[u][k] | code[u][k + 1] << 8);
+      if (WHOLE || (u < n && 32 * k < left)) to[32 * k] = from_f32<T>(two.x * f);
+      if (WHOLE || (u < n && 32 * (k + 1) < left)) to[32 * (k + 1)] = from_f32<T>(two.y * f);
+    }
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    decode_narrow_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales,
+                         uint64_t sld, uint64_t rows, uint32_t dim, uint32_t blocks, T* __restrict__ out,
+                         uint64_t stride, uint64_t step_rows, uint32_t step_blocks) {
+  constexpr uint32_t R = NARROW_ROWS;
+  const uint32_t lane = threadIdx.x & 31;
+  for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
+    const uint32_t b0 = it.block * BLOCK, c0 = b0 + lane;
+    const uint32_t n = static_cast<uint32_t>(min(static_cast<uint64_t>(R), rows - it.row));
+    const uint8_t* p = codes + it.row * ld + c0;
+    const uint8_t* s = scales + it.row * sld + it.block;
+    T* to = out + it.row * stride + c0;
+    if (n == R && b0 + BLOCK <= dim)
+      decode_narrow<T, true>(p, ld, s, sld, R, 0, to, stride);
+    else
+      decode_narrow<T, false>(p, ld, s, sld, n, c0 < dim ? dim - c0 : 0, to, stride);
   }
 }
 
@@ -123,15 +379,34 @@ static void with_type(int32_t dtype, F&& f) {
     f(static_cast<__nv_bfloat16*>(nullptr));
 }
 
+// Grid and step of the kernels above: items are a block of R rows, 8 a CTA at a time.
+struct Sweep {
+  unsigned grid;
+  uint64_t step_rows;
+  uint32_t step_blocks;
+  Sweep(const pxc_ctx* ctx, uint64_t rows, uint32_t blocks, uint32_t R) {
+    const uint64_t items = (rows + R - 1) / R * blocks;
+    grid = static_cast<unsigned>(std::min<uint64_t>((items + 7) / 8, static_cast<uint64_t>(ctx->sm_count) * 8));
+    step_rows = static_cast<uint64_t>(grid) * 8 / blocks * R;
+    step_blocks = grid * 8 % blocks;
+  }
+};
+
+// Whether every row starts on 16 bytes.
+static bool rows_wide(const void* p, uint64_t stride, int32_t dtype) {
+  return (reinterpret_cast<uintptr_t>(p) | stride * size_of(dtype)) % 16 == 0;
+}
+
 static void encode(pxc_ctx* ctx, const void* x, int32_t dtype, uint64_t stride, uint32_t dim, const pxc_bq_rows& out,
                    cudaStream_t s) {
   const uint32_t blocks = blocks_of(dim);
-  const unsigned grid =
-      static_cast<unsigned>(std::min<uint64_t>((out.rows * blocks + 7) / 8, static_cast<uint64_t>(ctx->sm_count) * 32));
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    encode_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(x), stride, out.rows, dim, blocks, out.codes, out.ld,
-                                          out.scales, out.sld);
+    const bool wide = rows_wide(x, stride, dtype);
+    const Sweep w(ctx, out.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS);
+    auto kernel = wide ? encode_wide_kernel<T> : encode_narrow_kernel<T>;
+    kernel<<<w.grid, 256, 0, s>>>(static_cast<const T*>(x), stride, out.rows, dim, blocks, out.codes, out.ld,
+                                  out.scales, out.sld, w.step_rows, w.step_blocks);
   });
   PXC_CUDA(cudaGetLastError());
   count_launch(ctx);
@@ -139,12 +414,14 @@ static void encode(pxc_ctx* ctx, const void* x, int32_t dtype, uint64_t stride, 
 
 static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out, int32_t dtype, uint64_t stride,
                    cudaStream_t s) {
-  const uint64_t quads = in.rows * ((dim + 3) / 4);
-  const unsigned grid =
-      static_cast<unsigned>(std::min<uint64_t>((quads + 255) / 256, static_cast<uint64_t>(ctx->sm_count) * 32));
+  const uint32_t blocks = blocks_of(dim);
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    decode_kernel<T><<<grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, static_cast<T*>(out), stride);
+    const bool wide = rows_wide(out, stride, dtype);
+    const Sweep w(ctx, in.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS);
+    auto kernel = wide ? decode_wide_kernel<T> : decode_narrow_kernel<T>;
+    kernel<<<w.grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, blocks, static_cast<T*>(out),
+                                  stride, w.step_rows, w.step_blocks);
   });
   PXC_CUDA(cudaGetLastError());
   count_launch(ctx);
