@@ -427,6 +427,17 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
   count_launch(ctx);
 }
 
+// Which shape of tile (bq_tc.cuh). Pairs where there are enough queries to be bound by the matrix
+// instructions and what feeds them.
+static bool pair_tiles(uint32_t q_rows, uint64_t rows) { return q_rows > 112 && rows > bq_tc::BM; }
+// Several times 128 rows where few queries leave a tile little work, and still eight tiles an SM.
+static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, int sms) {
+  const uint32_t most = q_rows <= 32 ? 4 : q_rows <= 64 ? 2 : 1;
+  for (uint32_t subs = most; subs > 1; subs /= 2)
+    if (rows >= static_cast<uint64_t>(subs) * bq_tc::BM * 8 * sms) return subs;
+  return 1;
+}
+
 static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, const Groups& g, void* out,
                     int32_t dtype, cudaStream_t s) {
   using namespace bq_tc;
@@ -442,33 +453,56 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   p.out = out;
   p.dim = dim;
   p.kblocks = blocks_of(dim);
-  uint64_t tiles;
-  if (!g.q_offsets) {
-    // the walk's even split: every tile but the last is this wide, one box brings it
-    const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
-    p.q_rows = p.q_box = static_cast<uint32_t>(up((q.rows + qt - 1) / qt, 16));
-    tiles = qt * ((b.rows + BM - 1) / BM);
+  // Queries of the widest tile: dense, the walk's even split; grouped, whatever a group may have.
+  const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
+  const bool dense = !g.q_offsets;
+  p.q_rows = static_cast<uint32_t>(dense ? up((q.rows + qt - 1) / qt, 16) : std::min<uint64_t>(MAX_Q, up(q.rows, 16)));
+  const bool pair = pair_tiles(p.q_rows, b.rows);
+  p.subs = dense && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
+  p.tile_rows = pair ? 2 * BM : p.subs * BM;
+  p.q_load = pair ? p.q_rows / 2 : p.q_rows;
+  if (dense) {
+    p.q_box = p.q_load;  // every tile but the last is this wide: one box brings it
   } else {
-    // groups of any size: room for the widest tile, filled by as many boxes as a tile needs
-    p.q_box = 32;
-    p.q_rows = static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, up(q.rows, 32)));
-    tiles = g.b_offsets ? ctx->sm_count : (g.groups + q.rows / MAX_Q) * ((g.n_each + BM - 1) / BM);
+    p.q_box = 32;  // as many boxes as a tile needs
+    p.q_load = static_cast<uint32_t>(up(p.q_load, 32));
   }
   p.wait_cycles = static_cast<uint64_t>(ctx->wait_ms) * 2000000ull;  // the SM clock is below 2 GHz
+  const uint32_t smem = plan(p);
   CUtensorMap map_b, map_q;
   make_tmap_u8_pitched(&map_b, b.codes, dim, b.ld, b.rows, BM);
   make_tmap_u8_pitched(&map_q, q.codes, dim, q.ld, q.rows, p.q_box);
-  const uint32_t smem = plan(p);
-  const unsigned grid = static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count, std::max<uint64_t>(tiles, 1)));
+  // no more CTAs than tiles, where the host can tell
+  uint64_t tiles = ctx->sm_count;
+  if (dense)
+    tiles = qt * ((b.rows + p.tile_rows - 1) / p.tile_rows);
+  else if (!g.b_offsets)
+    tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / MAX_Q) * ((g.n_each + p.tile_rows - 1) / p.tile_rows);
+  const uint32_t ctas = pair ? 2 : 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count / ctas, std::max<uint64_t>(tiles, 1))) * ctas);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = pair ? 1 : 0;
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (!(__atomic_load_n(&ctx->bq_ready, __ATOMIC_ACQUIRE) & (1u << dtype))) {  // once per context and type
-      PXC_CUDA(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
-      __atomic_fetch_or(&ctx->bq_ready, 1u << dtype, __ATOMIC_RELEASE);
+    auto kernel = pair          ? product_kernel<T, true, 1>
+                  : p.subs == 4 ? product_kernel<T, false, 4>
+                  : p.subs == 2 ? product_kernel<T, false, 2>
+                                : product_kernel<T, false, 1>;
+    const uint32_t bit = 1u << (4 * dtype + (pair ? 3 : p.subs / 2));
+    if (!(__atomic_load_n(&ctx->bq_ready, __ATOMIC_ACQUIRE) & bit)) {  // once per context and kernel
+      PXC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+      __atomic_fetch_or(&ctx->bq_ready, bit, __ATOMIC_RELEASE);
     }
-    product_kernel<T><<<grid, THREADS, smem, s>>>(map_b, map_q, p);
+    PXC_CUDA(cudaLaunchKernelEx(&config, kernel, map_b, map_q, p));
   });
-  PXC_CUDA(cudaGetLastError());
   count_launch(ctx);
 }
 

@@ -106,11 +106,12 @@ struct Tile {
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
 // matrix ends within the output. One that fails counts as empty and leaves a fault, so
 // that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
-template <uint32_t TQ, uint32_t TB>
+template <uint32_t TQ>
 struct Walk {
   static constexpr uint32_t PANEL = 64;
   const Groups& g;
   const uint32_t lane;
+  const uint32_t TB;  // base rows per tile
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
   uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
@@ -120,7 +121,10 @@ struct Walk {
   uint64_t gq = 0, gb = 0, gm = 0, gn = 0, first_value = 0;
   uint32_t qt = 0, bt = 0, width = 0;
 
-  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id) : g(groups), lane(lane_id) { load(); }
+  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t rows_per_tile)
+      : g(groups), lane(lane_id), TB(rows_per_tile) {
+    load();
+  }
 
   __device__ __forceinline__ static uint64_t scan(uint64_t v, uint32_t lane) {
 #pragma unroll
@@ -130,8 +134,9 @@ struct Walk {
     }
     return v;
   }
-  __device__ __forceinline__ static uint64_t tiles_of(uint64_t m, uint64_t n) {
-    return ((m + TQ - 1) / TQ) * ((n + TB - 1) / TB);
+  __device__ __forceinline__ uint64_t tiles_of(uint64_t m, uint64_t n) const {
+    // rows are below 2^31
+    return static_cast<uint64_t>((static_cast<uint32_t>(m) + TQ - 1) / TQ) * ((static_cast<uint32_t>(n) + TB - 1) / TB);
   }
 
   __device__ __forceinline__ void load() {
@@ -232,9 +237,10 @@ struct Walk {
     gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
     gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
     first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - gm * gn;
-    qt = static_cast<uint32_t>((gm + TQ - 1) / TQ), bt = static_cast<uint32_t>((gn + TB - 1) / TB);
+    const uint32_t m32 = static_cast<uint32_t>(gm);
+    qt = (m32 + TQ - 1) / TQ, bt = (static_cast<uint32_t>(gn) + TB - 1) / TB;
     // queries per tile: an even split, in steps of 16 (at most TQ, so that no tile is empty)
-    width = static_cast<uint32_t>(((gm + qt - 1) / qt + 15) / 16 * 16);
+    width = ((m32 + qt - 1) / qt + 15) / 16 * 16;
     last = tiles_before + __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
     first = last - static_cast<uint64_t>(qt) * bt;
     return true;

@@ -134,7 +134,7 @@ struct pxc_ctx {
   uint32_t* d_status = nullptr;  // [0] device error word, [1] aux
   uint32_t* h_status = nullptr;  // pinned mirror
   uint32_t* bq_faults = nullptr;  // pinned: failures that a block product's kernel left (bq.cuh)
-  uint32_t bq_ready = 0;          // block product kernels (a bit per output type) set up on the device
+  uint32_t bq_ready = 0;          // block product kernels (a bit each) set up on the device
   int sm_count = 0;
   bool profiling = false;
   unsigned long long launches = 0;  // kernels launched by this library on this context
