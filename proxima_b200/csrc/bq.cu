@@ -427,14 +427,12 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
   count_launch(ctx);
 }
 
-// Which shape of tile (bq_tc.cuh). Pairs where there are enough queries to be bound by the matrix
-// instructions and what feeds them.
-static bool pair_tiles(uint32_t q_rows, uint64_t rows) { return q_rows > 112 && rows > bq_tc::BM; }
-// Several times 128 rows where few queries leave a tile little work, and still eight tiles an SM.
-static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, int sms) {
-  const uint32_t most = q_rows <= 32 ? 4 : q_rows <= 64 ? 2 : 1;
-  for (uint32_t subs = most; subs > 1; subs /= 2)
-    if (rows >= static_cast<uint64_t>(subs) * bq_tc::BM * 8 * sms) return subs;
+// Several times 128 rows per tile where few queries leave a tile little work, as long as the rounds of
+// tiles over the SMs stay about as even.
+static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, uint64_t sms) {
+  const auto rounds = [&](uint64_t subs) { return up(up(rows, subs * bq_tc::BM) / (subs * bq_tc::BM), sms) / sms * subs; };
+  for (uint32_t subs = q_rows <= 48 ? 4 : q_rows <= 64 ? 2 : 1; subs > 1; subs /= 2)
+    if (rounds(subs) * 10 <= rounds(1) * 11) return subs;
   return 1;
 }
 
@@ -453,11 +451,15 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   p.out = out;
   p.dim = dim;
   p.kblocks = blocks_of(dim);
-  // Queries of the widest tile: dense, the walk's even split; grouped, whatever a group may have.
-  const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
+  // The widest tile: dense, the walk's even split; grouped, room for twice the mean, so that most groups
+  // are one tile and the rings stay deep.
   const bool dense = !g.q_offsets;
-  p.q_rows = static_cast<uint32_t>(dense ? up((q.rows + qt - 1) / qt, 16) : std::min<uint64_t>(MAX_Q, up(q.rows, 16)));
-  const bool pair = pair_tiles(p.q_rows, b.rows);
+  const uint64_t mean = q.rows / g.groups;
+  p.tile_q = dense ? MAX_Q : static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, std::max<uint64_t>(32, up(2 * mean, 32))));
+  const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
+  p.q_rows = dense ? static_cast<uint32_t>(up((q.rows + qt - 1) / qt, 16)) : p.tile_q;
+  // Pairs where there are enough queries to be bound by the matrix instructions and what feeds them.
+  const bool pair = p.q_rows > 112 && (dense ? b.rows > BM : mean > 112);
   p.subs = dense && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
   p.tile_rows = pair ? 2 * BM : p.subs * BM;
   p.q_load = pair ? p.q_rows / 2 : p.q_rows;
@@ -477,7 +479,7 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   if (dense)
     tiles = qt * ((b.rows + p.tile_rows - 1) / p.tile_rows);
   else if (!g.b_offsets)
-    tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / MAX_Q) * ((g.n_each + p.tile_rows - 1) / p.tile_rows);
+    tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / p.tile_q) * ((g.n_each + p.tile_rows - 1) / p.tile_rows);
   const uint32_t ctas = pair ? 2 : 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count / ctas, std::max<uint64_t>(tiles, 1))) * ctas);

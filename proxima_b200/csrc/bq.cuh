@@ -106,12 +106,11 @@ struct Tile {
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
 // matrix ends within the output. One that fails counts as empty and leaves a fault, so
 // that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
-template <uint32_t TQ>
 struct Walk {
   static constexpr uint32_t PANEL = 64;
   const Groups& g;
   const uint32_t lane;
-  const uint32_t TB;  // base rows per tile
+  const uint32_t TQ, TB;  // the most queries, and the base rows, of a tile
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
   uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
@@ -121,9 +120,20 @@ struct Walk {
   uint64_t gq = 0, gb = 0, gm = 0, gn = 0, first_value = 0;
   uint32_t qt = 0, bt = 0, width = 0;
 
-  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t rows_per_tile)
-      : g(groups), lane(lane_id), TB(rows_per_tile) {
+  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t queries, uint32_t rows)
+      : g(groups), lane(lane_id), TQ(queries), TB(rows) {
+    fetch(0);
     load();
+  }
+
+  // The offsets of the chunk from group `from` on, read ahead: the next chunk's are on their way while this
+  // one's tiles go out.
+  int64_t q_lo = 0, q_hi = 0, b_lo = 0, b_hi = 0;
+  __device__ __forceinline__ void fetch(uint64_t from) {
+    const uint64_t i = from + lane;
+    if (i >= g.groups) return;
+    if (g.q_offsets) q_lo = __ldg(g.q_offsets + i), q_hi = __ldg(g.q_offsets + i + 1);
+    if (g.b_offsets) b_lo = __ldg(g.b_offsets + i), b_hi = __ldg(g.b_offsets + i + 1);
   }
 
   __device__ __forceinline__ static uint64_t scan(uint64_t v, uint32_t lane) {
@@ -145,7 +155,7 @@ struct Walk {
     if (i < g.groups) {
       bool good = true;
       if (g.q_offsets) {
-        const int64_t lo = g.q_offsets[i], hi = g.q_offsets[i + 1];
+        const int64_t lo = q_lo, hi = q_hi;
         good = lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nq);
         q0 = static_cast<uint64_t>(lo);
         m = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
@@ -153,7 +163,7 @@ struct Walk {
         m = g.nq;
       }
       if (g.b_offsets) {
-        const int64_t lo = g.b_offsets[i], hi = g.b_offsets[i + 1];
+        const int64_t lo = b_lo, hi = b_hi;
         good = good && lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nb);
         b0 = static_cast<uint64_t>(lo);
         n = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
@@ -176,6 +186,7 @@ struct Walk {
       }
     }
     tiles_upto = scan(tiles_of(m, n), lane);
+    fetch(static_cast<uint64_t>(chunk) + 32);
   }
 
   // Tile number t, or false when there are fewer. All lanes call and get the same answer.

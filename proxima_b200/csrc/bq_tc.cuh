@@ -75,6 +75,7 @@ struct Params {
   void* out;
   uint64_t wait_cycles;
   uint32_t dim, kblocks;
+  uint32_t tile_q;     // the most queries of a tile
   uint32_t tile_rows;  // base rows per tile: BM * subs, or 2 * BM for a pair
   uint32_t subs;       // accumulators of a tile in this CTA
   uint32_t q_rows;     // queries of the widest tile, a multiple of 16
@@ -405,13 +406,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       Ring s, sf, acc, old;
       uint32_t quad = 0;  // number of the scale words; old: the slot of those SF_TMEM before
       bool ok = true;
-      const uint32_t base = smem_u32(smem), sf_base = smem_u32(sf_ring);
+      bool ready = false;  // the next stage is known to be full
+      const uint32_t sf_base = smem_u32(sf_ring);
+      const uint64_t desc_a = smem_desc_k_sw128(smem_u32(smem));
+      const uint64_t desc_b = smem_desc_k_sw128(smem_u32(smem) + subs * BASE_BYTES);
       const uint32_t last_steps = (p.dim - (kblocks - 1) * KB + MMA_K - 1) / MMA_K;
       while (ok && reader.next_one(t)) {
         const uint32_t width = round16(t.queries);
         if (!(ok = wait_one<PAIR>(c, &c.acc_empty[acc.i], acc.ph ^ 1, limit))) break;
         tc_fence_after();
-        const uint32_t d = tmem + acc.i * p.acc_cols;
+        const uint32_t d = tmem + acc.i * p.acc_cols, idesc0 = idesc_mxf8(G * BM, width, 0);
         for (uint32_t kb = 0; kb < kblocks; ++kb) {
           const uint32_t sfa = tmem + p.sf_col + (quad % SF_TMEM) * p.sf_cols, sfb = sfa + 4 * subs;
           if ((kb & 3) == 0) {
@@ -431,11 +435,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             copy_scales<G>(sfb, from + subs * ATOM);
             if (width > 128) copy_scales<G>(sfb + 4, from + (subs + 1) * ATOM);
           }
-          if (!(ok = wait_one(c, &c.full[s.i], s.ph, limit))) break;
+          if (!ready && !(ok = wait_one(c, &c.full[s.i], s.ph, limit))) break;
           tc_fence_after();
-          const uint64_t a = smem_desc_k_sw128(base + s.i * per_stage);
-          const uint64_t b = smem_desc_k_sw128(base + s.i * per_stage + subs * BASE_BYTES);
-          const uint32_t idesc = idesc_mxf8(G * BM, width, kb & 3);
+          // look at the next stage now: the answer is there once these MMAs are issued
+          Ring following = s;
+          following.step(p.stages);
+          ready = try_wait<false>(&c.full[following.i], following.ph);
+          const uint64_t at = static_cast<uint64_t>(s.i * (per_stage >> 4));
+          const uint64_t a = desc_a + at, b = desc_b + at;
+          const uint32_t idesc = idesc0 + ((kb & 3) << 4) + ((kb & 3) << 29);
           const uint32_t steps = kb + 1 == kblocks ? last_steps : KB / MMA_K;
 #pragma unroll
           for (uint32_t i = 0; i < subs; ++i) {
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             (kb | k) != 0);
           }
           commit<G>(&c.empty[s.i]);
-          s.step(p.stages);
+          s = following;
           if ((kb & 3) == 3 || kb + 1 == kblocks) {
             commit<G>(&c.sf_empty[sf.i]);
             ++quad;
@@ -505,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");  // landed before the CTA exits
   } else if (warp == 3) {
     // ---- the walk over tiles: the same in both CTAs of a pair ----
-    Walk<MAX_Q> walk(p.groups, lane, p.tile_rows);
+    Walk walk(p.groups, lane, p.tile_q, p.tile_rows);
     Ring s;
     for (uint64_t k = blockIdx.x / G;; k += gridDim.x / G) {
       const bool any = walk.find(k, t);
