@@ -534,6 +534,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (reader.next_warp(t)) {
       if (!wait_warp(c, &c.acc_full[acc.i], acc.ph, limit)) break;
       tc_fence_after();
+      // Outputs are stored with the streaming hint: without it a large one drives the operands out of L2
+      // (4096 x 65536 x 768 f32: 337 us, with it 290).
       // This warp's chunks of 32 columns, numbered through the subs: every other one. The accumulator goes
       // back once the last of them is in registers, before it is stored.
       const uint32_t chunks = (t.queries + 31) / 32, first = (warp - 4) >> 2, all = subs * chunks;
@@ -563,13 +565,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (q + 32 <= t.queries) {
 #pragma unroll
             for (uint32_t j = 0; j < 32; ++j) {
-              *dst[j & 3] = from_f32<T>(__uint_as_float(v[j]));
+              __stcs(dst[j & 3], from_f32<T>(__uint_as_float(v[j])));
               dst[j & 3] += stride4;
             }
           } else {
 #pragma unroll
             for (uint32_t j = 0; j < 32; ++j) {
-              if (q + j < t.queries) *dst[j & 3] = from_f32<T>(__uint_as_float(v[j]));
+              if (q + j < t.queries) __stcs(dst[j & 3], from_f32<T>(__uint_as_float(v[j])));
               dst[j & 3] += stride4;
             }
           }
