@@ -117,32 +117,33 @@ class BlockQuantizer:
             raise Configuration("device", index, f"the context is on device {self.ctx.device}")
         return _torch().current_stream(index) or 1
 
-    def _rows(self, c: BlockCodes, cuda: bool, name: str, device=None) -> N.PxcBqRows:
+    def _rows(self, c: BlockCodes, cuda: bool, name: str) -> N.PxcBqRows:
+        """The rows as the native calls take them: tensors on the context's device, or arrays."""
         if c.dim != self.dim:
             raise DimensionMismatch(self.dim, c.dim)
         codes, scales = c.codes, c.scales
-        if cuda:
-            if not (_is_cuda(codes) and _is_cuda(scales)) or codes.device != scales.device or (
-                    device is not None and codes.device != device):
-                raise Configuration(name, 0, "all operands on one device, or all on the host")
-            byte = _torch().uint8
-            (cr, cs), (sr, ss) = codes.stride() if codes.ndim == 2 else (0, 0), scales.stride() if scales.ndim == 2 else (0, 0)
-        else:
-            if _is_cuda(codes) or _is_cuda(scales):
-                raise Configuration(name, 0, "all operands on one device, or all on the host")
-            byte = np.uint8
-            (cr, cs), (sr, ss) = codes.strides if codes.ndim == 2 else (0, 0), scales.strides if scales.ndim == 2 else (0, 0)
-        if codes.dtype != byte or scales.dtype != byte or codes.ndim != 2 or scales.ndim != 2:
+        if _is_cuda(codes) != cuda or _is_cuda(scales) != cuda:
+            raise Configuration(name, 0, "all operands on one device, or all on the host")
+        if codes.ndim != 2 or scales.ndim != 2:
             raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
-        n, width = codes.shape
-        rows, blocks = scales.shape
+        if cuda:
+            byte, where, p, s = _torch().uint8, self.ctx.device, codes.data_ptr(), scales.data_ptr()
+            (cr, cs), (sr, ss) = codes.stride(), scales.stride()
+            if codes.get_device() != where or scales.get_device() != where:
+                raise Configuration("device", codes.get_device(), f"the context is on device {where}")
+        else:
+            byte, p, s = np.uint8, N.ptr(codes), N.ptr(scales)
+            (cr, cs), (sr, ss) = codes.strides, scales.strides
+        if codes.dtype != byte or scales.dtype != byte:
+            raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
+        (n, width), (rows, blocks) = codes.shape, scales.shape
         if rows != n or width < self._ld or blocks < self._sld:
             raise Configuration(name, n, f"codes are (n, >= {self._ld}) and scales (n, >= {self._sld}) here")
         if n <= 1:
             cr, sr = self._ld, self._sld
         if cs != 1 or ss != 1 or cr % 16 or sr % 4 or cr < self._ld or sr < self._sld:
             raise Configuration(name, n, "rows are contiguous, the codes' pitch a multiple of 16, the scales' of 4")
-        return N.PxcBqRows(N.ptr(codes), N.ptr(scales), n, cr, sr)
+        return N.PxcBqRows(p, s, n, cr, sr)
 
     def _vectors(self, vectors):
         """(n, dim), an array in one of the types."""
@@ -172,8 +173,8 @@ class BlockQuantizer:
             if (self.dim > 1 and step != 1) or (n > 1 and row < self.dim):
                 v = v.contiguous()
                 row = self.dim
-            codes = t.empty((n, ld), dtype=t.uint8, device=v.device)
-            scales = t.empty((n, sld), dtype=t.uint8, device=v.device)
+            codes = t.empty(n, ld, dtype=t.uint8, device=v.device)
+            scales = codes.new_empty(n, sld)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
             t.encode(self.ctx.handle, v.data_ptr(), code, row if n > 1 else self.dim, self.dim, C.byref(rows), stream)
             return BlockCodes(codes, scales, self.dim)
@@ -190,7 +191,7 @@ class BlockQuantizer:
         if cuda:
             t = _torch()
             code = _dtype_code(dtype or t.float32)
-            out = t.empty((rows.rows, self.dim), dtype=dtype or t.float32, device=codes.codes.device)
+            out = t.empty(rows.rows, self.dim, dtype=dtype or t.float32, device=codes.codes.device)
             t.decode(self.ctx.handle, C.byref(rows), self.dim, out.data_ptr(), code, self.dim, self._stream(out))
             return out
         out = np.zeros((len(codes), self.dim), dtype or np.float32)
@@ -202,15 +203,14 @@ class BlockQuantizer:
         """The dot product of every pair of rows, (nq, n): f32 sums, rounded once to ``dtype``
         (float32). ``out`` may be a tensor to write into, its rows strided."""
         cuda = _is_cuda(queries.codes)
-        dev = queries.codes.device if cuda else None
-        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base", dev)
+        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base")
         shape = (q.rows, b.rows)
         if cuda:
-            t = _torch()
+            t, dev = _torch(), queries.codes.device
             stride = shape[1] or 1
             if out is None:
                 code = _dtype_code(dtype or t.float32)
-                out = t.empty(shape, dtype=dtype or t.float32, device=dev)
+                out = t.empty(*shape, dtype=dtype or t.float32, device=dev)
             else:
                 if (tuple(out.shape) != shape or out.device != dev or (dtype is not None and out.dtype != dtype)
                         or (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1])):
@@ -237,8 +237,8 @@ class BlockQuantizer:
         offsets back to find it waits for the device)."""
         cuda = _is_cuda(queries.codes)
         dev = queries.codes.device if cuda else None
-        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base", dev)
-        qo, bo = (self._offsets(o, cuda, dev) for o in (query_offsets, base_offsets))
+        q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base")
+        qo, bo = self._offsets(query_offsets, cuda, dev), self._offsets(base_offsets, cuda, dev)
         if qo is None or len(qo) < 2 or (bo is not None and len(bo) != len(qo)):
             raise Configuration("offsets", 0, "groups + 1 int64 values for the queries, and for the base where given")
         groups = len(qo) - 1
@@ -257,7 +257,7 @@ class BlockQuantizer:
         if cuda:
             t = _torch()
             code = _dtype_code(dtype or t.float32)
-            out = t.empty(shape, dtype=dtype or t.float32, device=dev)
+            out = t.empty(*shape, dtype=dtype or t.float32, device=dev)
             t.grouped(self.ctx.handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups, self.dim, out.data_ptr(),
                       code, size, self._stream(out))
             return out
