@@ -482,6 +482,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           sf.step(p.sf_slots);
         }
       }
+      // the leader's signals to this CTA are on their way until its last one is here
+      wait_drained(&c.done, 0, limit);
     }
   } else if (warp == 2) {
     // ---- scales ----
