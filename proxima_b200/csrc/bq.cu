@@ -23,8 +23,10 @@ static uint32_t blocks_of(uint32_t dim) { return (dim + BLOCK - 1) / BLOCK; }
 // moves 16 bytes of vector at a time, and what is done once per block (the reduction, the scale, the
 // addresses) is done for four. Items go by a fixed step: no division stands in the loop.
 //
-// Where rows do not start on 16 bytes (an odd pitch or base), a whole warp takes a block, its lanes single
-// components 32 apart: each access covers neighbouring bytes, and whole sectors of the codes.
+// Where rows do not start on 16 bytes (an odd pitch or base), the encoder gathers the same 16 bytes from
+// narrower loads, none of which leaves them. The decoder gives a whole warp to a block then, its lanes 32
+// apart, so that each store covers neighbouring bytes: partial sectors would each be written several
+// times over.
 
 // The items of one warp: a block of the R rows from `row` on.
 template <uint32_t R>
@@ -100,9 +102,26 @@ __device__ __forceinline__ void store_scale(uint8_t* row, uint32_t block, uint32
   }
 }
 
+// 16 bytes of components from any address that is aligned to one: 16-bit types by the three words that lie
+// on word boundaries and the two components around or behind them.
 template <class T>
+__device__ __forceinline__ uint4 gather(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+    return make_uint4(__ldcs(w), __ldcs(w + 1), __ldcs(w + 2), __ldcs(w + 3));
+  } else {
+    const uint32_t odd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) >> 1) & 1u, shift = 16 * odd;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p + odd);
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], h0 = h[odd ? 0 : 6], h7 = h[7];
+    return make_uint4(__funnelshift_l(h0 << 16, w0, shift), __funnelshift_l(w0, w1, shift),
+                      __funnelshift_l(w1, w2, shift), __funnelshift_l(w2, odd ? h7 : h0 | h7 << 16, shift));
+  }
+}
+
+template <class T, bool WIDE>
 __global__ void __launch_bounds__(256)
-    encode_wide_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
+    encode_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
                        uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld,
                        uint64_t step_rows, uint32_t step_blocks) {
   constexpr uint32_t V = CHUNK<T>, C = 16 / V, R = WIDE_ROWS<T>, U = R / 4;
@@ -118,7 +137,12 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (uint32_t k = 0; k < C; ++k) {
         uint4 q = make_uint4(0, 0, 0, 0);
-        if (r < rows && c0 + k * 8 * V + V <= dim) q = __ldcs(reinterpret_cast<const uint4*>(p + k * 8 * V));
+        if (r < rows && c0 + k * 8 * V + V <= dim) {
+          if constexpr (WIDE)
+            q = __ldcs(reinterpret_cast<const uint4*>(p + k * 8 * V));
+          else
+            q = gather<T>(p + k * 8 * V);
+        }
         unpack<T>(q, v[u][k]);
       }
     }
@@ -177,58 +201,6 @@ __global__ void __launch_bounds__(256)
         if (l == 0) store_scale(scales + r * sld, it.block, blocks, byte);
       }
     }
-  }
-}
-
-// One item; WHOLE: all rows and the whole block are there, so nothing is tested.
-template <class T, bool WHOLE>
-__device__ __forceinline__ void encode_narrow(const T* __restrict__ p, uint64_t stride, uint32_t n, uint32_t left,
-                                              uint32_t code_left, uint8_t* __restrict__ to, uint64_t ld,
-                                              uint8_t* __restrict__ s, uint64_t sld, uint32_t block, uint32_t blocks,
-                                              uint32_t lane) {
-  constexpr uint32_t R = NARROW_ROWS;
-  float v[R][4];
-#pragma unroll
-  for (uint32_t u = 0; u < R; ++u, p += stride)
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) v[u][k] = WHOLE || (u < n && 32 * k < left) ? to_f32<T>(p[32 * k]) : 0.0f;
-#pragma unroll
-  for (uint32_t u = 0; u < R; ++u, to += ld, s += sld) {
-    const float most = fmaxf(fmaxf(fabsf(v[u][0]), fabsf(v[u][1])), fmaxf(fabsf(v[u][2]), fabsf(v[u][3])));
-    uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most));
-    if (top >= 0x7F800000u)
-      top = __reduce_max_sync(0xFFFFFFFFu, max(max(finite_bits(v[u][0]), finite_bits(v[u][1])),
-                                               max(finite_bits(v[u][2]), finite_bits(v[u][3]))));
-    const uint32_t byte = scale_byte(top);
-    const float f = inverse_scale(byte);
-    const uint32_t four = to_codes(v[u][0] * f, v[u][1] * f, v[u][2] * f, v[u][3] * f);
-    if (WHOLE || u < n) {
-#pragma unroll
-      for (uint32_t k = 0; k < 4; ++k)
-        if (WHOLE || 32 * k < code_left) to[32 * k] = static_cast<uint8_t>(four >> (8 * k));
-      if (lane == 0) store_scale(s, block, blocks, byte);
-    }
-  }
-}
-
-template <class T>
-__global__ void __launch_bounds__(256)
-    encode_narrow_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
-                         uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld,
-                         uint64_t step_rows, uint32_t step_blocks) {
-  constexpr uint32_t R = NARROW_ROWS;
-  const uint32_t lane = threadIdx.x & 31, code_end = (dim + 15) / 16 * 16;
-  for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
-    const uint32_t b0 = it.block * BLOCK, c0 = b0 + lane;  // components c0 + 32 k
-    const uint32_t n = static_cast<uint32_t>(min(static_cast<uint64_t>(R), rows - it.row));
-    const T* p = x + it.row * stride + c0;
-    uint8_t* to = codes + it.row * ld + c0;
-    uint8_t* s = scales + it.row * sld;
-    if (n == R && b0 + BLOCK <= dim)
-      encode_narrow<T, true>(p, stride, R, 0, 0, to, ld, s, sld, it.block, blocks, lane);
-    else
-      encode_narrow<T, false>(p, stride, n, c0 < dim ? dim - c0 : 0, c0 < code_end ? code_end - c0 : 0, to, ld, s, sld,
-                              it.block, blocks, lane);
   }
 }
 
@@ -321,10 +293,10 @@ __global__ void __launch_bounds__(256)
     const uint8_t* p = codes + it.row * ld + c0;
     const uint8_t* s = scales + it.row * sld + it.block;
     T* to = out + it.row * stride + c0;
-    if (n == R && b0 + BLOCK <= dim)
-      decode_narrow<T, true>(p, ld, s, sld, R, 0, to, stride);
-    else
+    if (n < R || b0 + BLOCK > dim)
       decode_narrow<T, false>(p, ld, s, sld, n, c0 < dim ? dim - c0 : 0, to, stride);
+    else
+      decode_narrow<T, true>(p, ld, s, sld, R, 0, to, stride);
   }
 }
 
@@ -379,14 +351,16 @@ static void with_type(int32_t dtype, F&& f) {
     f(static_cast<__nv_bfloat16*>(nullptr));
 }
 
-// Grid and step of the kernels above: items are a block of R rows, 8 a CTA at a time.
+// Grid and step of the kernels above: items are a block of R rows, 8 a CTA at a time. Many short CTAs even out
+// the SMs' shares where a warp moves few bytes at a time (decode 1M x 128 to f32: 8 an SM 110 us, 64
+// 97 us); 16-bit vectors are encoded by long ones (8192 x 4096 bf16: 21 us, with 64 23 us).
 struct Sweep {
   unsigned grid;
   uint64_t step_rows;
   uint32_t step_blocks;
-  Sweep(const pxc_ctx* ctx, uint64_t rows, uint32_t blocks, uint32_t R) {
+  Sweep(const pxc_ctx* ctx, uint64_t rows, uint32_t blocks, uint32_t R, uint32_t per_sm) {
     const uint64_t items = (rows + R - 1) / R * blocks;
-    grid = static_cast<unsigned>(std::min<uint64_t>((items + 7) / 8, static_cast<uint64_t>(ctx->sm_count) * 8));
+    grid = static_cast<unsigned>(std::min<uint64_t>((items + 7) / 8, static_cast<uint64_t>(ctx->sm_count) * per_sm));
     step_rows = static_cast<uint64_t>(grid) * 8 / blocks * R;
     step_blocks = grid * 8 % blocks;
   }
@@ -402,9 +376,8 @@ static void encode(pxc_ctx* ctx, const void* x, int32_t dtype, uint64_t stride, 
   const uint32_t blocks = blocks_of(dim);
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool wide = rows_wide(x, stride, dtype);
-    const Sweep w(ctx, out.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS);
-    auto kernel = wide ? encode_wide_kernel<T> : encode_narrow_kernel<T>;
+    const Sweep w(ctx, out.rows, blocks, WIDE_ROWS<T>, sizeof(T) == 4 ? 64 : 8);
+    auto kernel = rows_wide(x, stride, dtype) ? encode_kernel<T, true> : encode_kernel<T, false>;
     kernel<<<w.grid, 256, 0, s>>>(static_cast<const T*>(x), stride, out.rows, dim, blocks, out.codes, out.ld,
                                   out.scales, out.sld, w.step_rows, w.step_blocks);
   });
@@ -418,7 +391,7 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const bool wide = rows_wide(out, stride, dtype);
-    const Sweep w(ctx, in.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS);
+    const Sweep w(ctx, in.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS, 64);
     auto kernel = wide ? decode_wide_kernel<T> : decode_narrow_kernel<T>;
     kernel<<<w.grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, blocks, static_cast<T*>(out),
                                   stride, w.step_rows, w.step_blocks);
