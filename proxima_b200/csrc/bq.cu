@@ -434,7 +434,8 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   // Pairs where there are enough queries to be bound by the matrix instructions and what feeds them.
   const bool pair = p.q_rows > 112 && (dense ? b.rows > BM : mean > 112);
   p.subs = dense && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
-  p.tile_rows = pair ? 2 * BM : p.subs * BM;
+  const uint32_t tile_rows = pair ? 2 * BM : p.subs * BM;
+  p.tile_log2 = tile_rows == BM ? 7 : tile_rows == 2 * BM ? 8 : 9;
   p.q_load = pair ? p.q_rows / 2 : p.q_rows;
   if (dense) {
     p.q_box = p.q_load;  // every tile but the last is this wide: one box brings it
@@ -450,9 +451,9 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   // no more CTAs than tiles, where the host can tell
   uint64_t tiles = ctx->sm_count;
   if (dense)
-    tiles = qt * ((b.rows + p.tile_rows - 1) / p.tile_rows);
+    tiles = qt * ((b.rows + tile_rows - 1) / tile_rows);
   else if (!g.b_offsets)
-    tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / p.tile_q) * ((g.n_each + p.tile_rows - 1) / p.tile_rows);
+    tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / p.tile_q) * ((g.n_each + tile_rows - 1) / tile_rows);
   const uint32_t ctas = pair ? 2 : 1;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(std::min<uint64_t>(ctx->sm_count / ctas, std::max<uint64_t>(tiles, 1))) * ctas);

@@ -106,22 +106,25 @@ struct Tile {
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
 // matrix ends within the output. One that fails counts as empty and leaves a fault, so
 // that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
+//
+// A new group costs a few hundred cycles of one warp (32-bit scans and shuffles wherever the numbers
+// allow): short groups come at one a tile, and their loads wait for the walk.
 struct Walk {
   static constexpr uint32_t PANEL = 64;
   const Groups& g;
   const uint32_t lane;
-  const uint32_t TQ, TB;  // the most queries, and the base rows, of a tile
+  const uint32_t TQ, tb_log2;  // the most queries of a tile; its base rows are a power of two
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
   uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
-  uint64_t q0 = 0, b0 = 0, m = 0, n = 0;
+  uint32_t q0 = 0, b0 = 0, m = 0, n = 0;
   // the group found last, in every lane: its tiles are [first, last)
-  uint64_t first = 0, last = 0;
-  uint64_t gq = 0, gb = 0, gm = 0, gn = 0, first_value = 0;
+  uint64_t first = 0, last = 0, first_value = 0;
+  uint32_t gq = 0, gb = 0, gm = 0, gn = 0;
   uint32_t qt = 0, bt = 0, width = 0;
 
-  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t queries, uint32_t rows)
-      : g(groups), lane(lane_id), TQ(queries), TB(rows) {
+  __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t queries, uint32_t rows_log2)
+      : g(groups), lane(lane_id), TQ(queries), tb_log2(rows_log2) {
     fetch(0);
     load();
   }
@@ -136,17 +139,24 @@ struct Walk {
     if (g.b_offsets) b_lo = __ldg(g.b_offsets + i), b_hi = __ldg(g.b_offsets + i + 1);
   }
 
-  __device__ __forceinline__ static uint64_t scan(uint64_t v, uint32_t lane) {
+  template <class U>
+  __device__ __forceinline__ static U scan_as(U v, uint32_t lane) {
 #pragma unroll
     for (uint32_t d = 1; d < 32; d <<= 1) {
-      const uint64_t u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      const U u = __shfl_up_sync(0xFFFFFFFFu, v, d);
       if (lane >= d) v += u;
     }
     return v;
   }
-  __device__ __forceinline__ uint64_t tiles_of(uint64_t m, uint64_t n) const {
-    // rows are below 2^31
-    return static_cast<uint64_t>((static_cast<uint32_t>(m) + TQ - 1) / TQ) * ((static_cast<uint32_t>(n) + TB - 1) / TB);
+  __device__ __forceinline__ uint64_t scan(uint64_t v) const {
+    if (__any_sync(0xFFFFFFFFu, v >> 26 != 0)) return scan_as<uint64_t>(v, lane);
+    return scan_as<uint32_t>(static_cast<uint32_t>(v), lane);
+  }
+  __device__ __forceinline__ uint32_t query_tiles(uint32_t queries) const {
+    return queries <= TQ ? (queries != 0) : (queries + TQ - 1) / TQ;
+  }
+  __device__ __forceinline__ uint32_t base_tiles(uint32_t rows) const {
+    return (rows + (1u << tb_log2) - 1) >> tb_log2;
   }
 
   __device__ __forceinline__ void load() {
@@ -155,21 +165,19 @@ struct Walk {
     if (i < g.groups) {
       bool good = true;
       if (g.q_offsets) {
-        const int64_t lo = q_lo, hi = q_hi;
-        good = lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nq);
-        q0 = static_cast<uint64_t>(lo);
-        m = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
+        good = q_lo >= 0 && q_hi >= q_lo && q_hi <= static_cast<int64_t>(g.nq);
+        q0 = static_cast<uint32_t>(q_lo);
+        m = static_cast<uint32_t>(q_hi) - q0;
       } else {
-        m = g.nq;
+        m = static_cast<uint32_t>(g.nq);
       }
       if (g.b_offsets) {
-        const int64_t lo = b_lo, hi = b_hi;
-        good = good && lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(g.nb);
-        b0 = static_cast<uint64_t>(lo);
-        n = static_cast<uint64_t>(hi) - static_cast<uint64_t>(lo);
+        good = good && b_lo >= 0 && b_hi >= b_lo && b_hi <= static_cast<int64_t>(g.nb);
+        b0 = static_cast<uint32_t>(b_lo);
+        n = static_cast<uint32_t>(b_hi) - b0;
       } else {
-        b0 = i * g.n_each;
-        n = g.n_each;
+        b0 = i * static_cast<uint32_t>(g.n_each);
+        n = static_cast<uint32_t>(g.n_each);
       }
       if (!good) {
         leave_fault(g.faults, FAULT_OFFSETS);
@@ -179,13 +187,13 @@ struct Walk {
     if (g.b_offsets) {
       // m, n < 2^31 and size <= 2^48: with each term held to size + 1 no sum overflows, and one
       // that is past the room stays past it for all groups behind
-      values_upto = scan(min(m * n, g.size + 1), lane);
-      if (m * n != 0 && values_before + values_upto > g.size) {
+      values_upto = scan(min(static_cast<uint64_t>(m) * n, g.size + 1));
+      if (m != 0 && n != 0 && values_before + values_upto > g.size) {
         leave_fault(g.faults, FAULT_OFFSETS);
         m = 0;
       }
     }
-    tiles_upto = scan(tiles_of(m, n), lane);
+    tiles_upto = scan(static_cast<uint64_t>(query_tiles(m)) * base_tiles(n));
     fetch(static_cast<uint64_t>(chunk) + 32);
   }
 
@@ -194,18 +202,16 @@ struct Walk {
     if (t >= last && !enter(t)) return false;
     const uint64_t r = t - first;
     uint32_t qi, bi;
-    if (last - first <= 0xFFFFFFFFu) {
+    if (qt == 1) {
+      qi = 0, bi = static_cast<uint32_t>(r);
+    } else if (last - first <= 0xFFFFFFFFu) {
       const uint32_t r32 = static_cast<uint32_t>(r);
-      if (qt == 1) {
-        qi = 0, bi = r32;
-      } else {
-        // at most 2^32 / bt tiles of queries, so a panel's PANEL * qt tiles fit 32 bits whenever bt >= PANEL
-        const uint32_t panel = bt <= PANEL ? 0 : r32 / (PANEL * qt);
-        const uint32_t in_panel = r32 - panel * PANEL * qt;
-        const uint32_t across = min(PANEL, bt - panel * PANEL);
-        qi = in_panel / across;
-        bi = panel * PANEL + in_panel - qi * across;
-      }
+      // at most 2^32 / bt tiles of queries, so a panel's PANEL * qt tiles fit 32 bits whenever bt >= PANEL
+      const uint32_t panel = bt <= PANEL ? 0 : r32 / (PANEL * qt);
+      const uint32_t in_panel = r32 - panel * PANEL * qt;
+      const uint32_t across = min(PANEL, bt - panel * PANEL);
+      qi = in_panel / across;
+      bi = panel * PANEL + in_panel - qi * across;
     } else {
       const uint32_t panel = static_cast<uint32_t>(r / (static_cast<uint64_t>(PANEL) * qt));
       const uint64_t in_panel = r - static_cast<uint64_t>(panel) * PANEL * qt;
@@ -213,17 +219,17 @@ struct Walk {
       qi = static_cast<uint32_t>(in_panel / across);
       bi = panel * PANEL + static_cast<uint32_t>(in_panel - static_cast<uint64_t>(qi) * across);
     }
-    const uint64_t qa = static_cast<uint64_t>(qi) * width, ba = static_cast<uint64_t>(bi) * TB;
-    out.q0 = static_cast<uint32_t>(gq + qa);
-    out.queries = static_cast<uint32_t>(min(static_cast<uint64_t>(width), gm - qa));
-    out.b0 = static_cast<uint32_t>(gb + ba);
-    out.rows = static_cast<uint32_t>(min(static_cast<uint64_t>(TB), gn - ba));
+    const uint32_t qa = qi * width, ba = bi << tb_log2;  // below gm and gn
+    out.q0 = gq + qa;
+    out.queries = min(width, gm - qa);
+    out.b0 = gb + ba;
+    out.rows = min(1u << tb_log2, gn - ba);
     if (g.b_offsets) {
       out.stride = gn;
-      out.at = first_value + qa * gn + ba;
+      out.at = first_value + static_cast<uint64_t>(qa) * gn + ba;
     } else {
       out.stride = g.stride;
-      out.at = (gq + qa) * g.stride + ba;
+      out.at = static_cast<uint64_t>(gq + qa) * g.stride + ba;
     }
     return true;
   }
@@ -247,11 +253,10 @@ struct Walk {
     const uint32_t who = __ffs(__ballot_sync(0xFFFFFFFFu, t < tiles_before + tiles_upto)) - 1;
     gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
     gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
-    first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - gm * gn;
-    const uint32_t m32 = static_cast<uint32_t>(gm);
-    qt = (m32 + TQ - 1) / TQ, bt = (static_cast<uint32_t>(gn) + TB - 1) / TB;
+    first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - static_cast<uint64_t>(gm) * gn;
+    qt = query_tiles(gm), bt = base_tiles(gn);
     // queries per tile: an even split, in steps of 16 (at most TQ, so that no tile is empty)
-    width = ((m32 + qt - 1) / qt + 15) / 16 * 16;
+    width = ((qt == 1 ? gm : (gm + qt - 1) / qt) + 15) / 16 * 16;
     last = tiles_before + __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
     first = last - static_cast<uint64_t>(qt) * bt;
     return true;

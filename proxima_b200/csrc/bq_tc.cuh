@@ -76,7 +76,7 @@ struct Params {
   uint64_t wait_cycles;
   uint32_t dim, kblocks;
   uint32_t tile_q;     // the most queries of a tile
-  uint32_t tile_rows;  // base rows per tile: BM * subs, or 2 * BM for a pair
+  uint32_t tile_log2;  // log2 of its base rows: BM * subs, or 2 * BM for a pair
   uint32_t subs;       // accumulators of a tile in this CTA
   uint32_t q_rows;     // queries of the widest tile, a multiple of 16
   uint32_t q_load;     // and those of them that a stage of this CTA has room for
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");  // landed before the CTA exits
   } else if (warp == 3) {
     // ---- the walk over tiles: the same in both CTAs of a pair ----
-    Walk walk(p.groups, lane, p.tile_q, p.tile_rows);
+    Walk walk(p.groups, lane, p.tile_q, p.tile_log2);
     Ring s;
     for (uint64_t k = blockIdx.x / G;; k += gridDim.x / G) {
       const bool any = walk.find(k, t);
