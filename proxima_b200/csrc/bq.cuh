@@ -81,8 +81,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 // (`groups` + 1 each); without base offsets every group has n_each rows and the output is
 // indexed by query, else the groups' matrices follow one another.
 struct Groups {
-  const int64_t* q_offsets;  // NULL: dense
-  const int64_t* b_offsets;  // NULL: even
+  const int64_t* q_offsets;  // NULL: dense, one group
+  const int64_t* b_offsets;  // NULL: even (or dense)
   uint32_t groups;
   uint64_t nq, nb;      // rows on either side
   uint64_t n_each;      // even (and dense): base rows per group, and the output's row pitch is `stride`
@@ -97,27 +97,30 @@ struct Tile {
   uint64_t at, stride;
 };
 
-// Walks the tiles in order, a warp at a time: lane i holds group chunk + i. Tiles are numbered
-// through the groups; find() is called with rising numbers, so that each chunk of 32 groups is
-// read once. Inside a group the base rows come in panels of PANEL tiles, all queries against
-// one panel before the next: neighbouring CTAs write neighbouring columns of the same
-// output rows, and a panel's rows stay in L2 while the queries pass.
+// Walks the tiles in order, a warp at a time: a chunk of 128 groups, four to a lane. Tiles are numbered
+// through the groups; find() is called with rising numbers, so that each chunk is read once, and the next
+// one's offsets are on their way meanwhile. Short groups come at one a tile and more, so what a chunk and a
+// group cost counts: 32-bit scans and shuffles wherever the numbers allow, and no division for a
+// group of one tile of queries.
+//
+// Inside a group the base rows come in panels of PANEL tiles, all queries against one panel before the
+// next: neighbouring CTAs write neighbouring columns of the same output rows, and a panel's rows stay in
+// L2 while the queries pass.
 //
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
 // matrix ends within the output. One that fails counts as empty and leaves a fault, so
 // that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
-//
-// A new group costs a few hundred cycles of one warp (32-bit scans and shuffles wherever the numbers
-// allow): short groups come at one a tile, and their loads wait for the walk.
 struct Walk {
-  static constexpr uint32_t PANEL = 64;
+  static constexpr uint32_t PANEL = 64, PER = 4, CHUNK = 32 * PER;
   const Groups& g;
   const uint32_t lane;
   const uint32_t TQ, tb_log2;  // the most queries of a tile; its base rows are a power of two
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
-  uint64_t tiles_upto = 0, values_upto = 0;      // inclusive scans over this chunk
-  uint32_t q0 = 0, b0 = 0, m = 0, n = 0;
+  uint64_t tiles_upto = 0, values_upto = 0;      // of this one, up to and with this lane's groups
+  // this lane's groups: first rows, sizes, tiles and output values
+  uint32_t q0[PER], b0[PER], m[PER], n[PER];
+  uint64_t tiles[PER], values[PER];
   // the group found last, in every lane: its tiles are [first, last)
   uint64_t first = 0, last = 0, first_value = 0;
   uint32_t gq = 0, gb = 0, gm = 0, gn = 0;
@@ -125,18 +128,33 @@ struct Walk {
 
   __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t queries, uint32_t rows_log2)
       : g(groups), lane(lane_id), TQ(queries), tb_log2(rows_log2) {
-    fetch(0);
-    load();
+    if (g.q_offsets) {
+      fetch(0);
+      load();
+    } else {  // dense: one group of everything
+      chunk = g.groups;
+      gm = static_cast<uint32_t>(g.nq), gn = static_cast<uint32_t>(g.nb);
+      split();
+    }
   }
 
-  // The offsets of the chunk from group `from` on, read ahead: the next chunk's are on their way while this
-  // one's tiles go out.
-  int64_t q_lo = 0, q_hi = 0, b_lo = 0, b_hi = 0;
+  // The group's tiles from `first` on: an even split of its queries in steps of 16 (at most TQ, so that no tile is
+  // empty).
+  __device__ __forceinline__ void split() {
+    qt = query_tiles(gm), bt = base_tiles(gn);
+    width = ((qt == 1 ? gm : (gm + qt - 1) / qt) + 15) / 16 * 16;
+    last = first + static_cast<uint64_t>(qt) * bt;
+  }
+
+  // The offsets around this lane's groups of the chunk from group `from` on; behind the last group, its end.
+  int64_t q_next[PER + 1], b_next[PER + 1];
   __device__ __forceinline__ void fetch(uint64_t from) {
-    const uint64_t i = from + lane;
-    if (i >= g.groups) return;
-    if (g.q_offsets) q_lo = __ldg(g.q_offsets + i), q_hi = __ldg(g.q_offsets + i + 1);
-    if (g.b_offsets) b_lo = __ldg(g.b_offsets + i), b_hi = __ldg(g.b_offsets + i + 1);
+#pragma unroll
+    for (uint32_t j = 0; j <= PER; ++j) {
+      const uint64_t i = min(from + lane * PER + j, static_cast<uint64_t>(g.groups));
+      q_next[j] = __ldg(g.q_offsets + i);
+      b_next[j] = g.b_offsets ? __ldg(g.b_offsets + i) : 0;
+    }
   }
 
   template <class U>
@@ -158,43 +176,47 @@ struct Walk {
   __device__ __forceinline__ uint32_t base_tiles(uint32_t rows) const {
     return (rows + (1u << tb_log2) - 1) >> tb_log2;
   }
+  __device__ __forceinline__ static bool within(int64_t lo, int64_t hi, uint64_t rows) {
+    return lo >= 0 && hi >= lo && hi <= static_cast<int64_t>(rows);
+  }
 
   __device__ __forceinline__ void load() {
-    const uint32_t i = chunk + lane;
-    q0 = b0 = m = n = 0;
-    if (i < g.groups) {
-      bool good = true;
-      if (g.q_offsets) {
-        good = q_lo >= 0 && q_hi >= q_lo && q_hi <= static_cast<int64_t>(g.nq);
-        q0 = static_cast<uint32_t>(q_lo);
-        m = static_cast<uint32_t>(q_hi) - q0;
-      } else {
-        m = static_cast<uint32_t>(g.nq);
-      }
-      if (g.b_offsets) {
-        good = good && b_lo >= 0 && b_hi >= b_lo && b_hi <= static_cast<int64_t>(g.nb);
-        b0 = static_cast<uint32_t>(b_lo);
-        n = static_cast<uint32_t>(b_hi) - b0;
-      } else {
-        b0 = i * static_cast<uint32_t>(g.n_each);
-        n = static_cast<uint32_t>(g.n_each);
-      }
-      if (!good) {
-        leave_fault(g.faults, FAULT_OFFSETS);
-        q0 = b0 = m = n = 0;
-      }
+    bool bad = false;
+    uint64_t value_sum = 0, tile_sum = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      const uint64_t i = static_cast<uint64_t>(chunk) + lane * PER + j;
+      const bool there = i < g.groups;
+      q0[j] = static_cast<uint32_t>(q_next[j]);
+      m[j] = static_cast<uint32_t>(q_next[j + 1]) - q0[j];
+      b0[j] = g.b_offsets ? static_cast<uint32_t>(b_next[j]) : static_cast<uint32_t>(i * g.n_each);
+      n[j] = g.b_offsets ? static_cast<uint32_t>(b_next[j + 1]) - b0[j] : there ? static_cast<uint32_t>(g.n_each) : 0u;
+      const bool good =
+          within(q_next[j], q_next[j + 1], g.nq) && (!g.b_offsets || within(b_next[j], b_next[j + 1], g.nb));
+      if (!good) m[j] = n[j] = 0;
+      bad = bad || (there && !good);
+      // m, n < 2^31 and size <= 2^48: with each term held to size + 1 no sum overflows, and one that is past the
+      // room stays past it for all groups behind
+      values[j] = g.b_offsets ? min(static_cast<uint64_t>(m[j]) * n[j], g.size + 1) : 0;
+      value_sum += values[j];
     }
     if (g.b_offsets) {
-      // m, n < 2^31 and size <= 2^48: with each term held to size + 1 no sum overflows, and one
-      // that is past the room stays past it for all groups behind
-      values_upto = scan(min(static_cast<uint64_t>(m) * n, g.size + 1));
-      if (m != 0 && n != 0 && values_before + values_upto > g.size) {
-        leave_fault(g.faults, FAULT_OFFSETS);
-        m = 0;
+      values_upto = scan(value_sum);
+      uint64_t upto = values_before + values_upto - value_sum;
+#pragma unroll
+      for (uint32_t j = 0; j < PER; ++j) {
+        upto += values[j];
+        if (values[j] != 0 && upto > g.size) bad = true, m[j] = 0;
       }
     }
-    tiles_upto = scan(static_cast<uint64_t>(query_tiles(m)) * base_tiles(n));
-    fetch(static_cast<uint64_t>(chunk) + 32);
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      tiles[j] = static_cast<uint64_t>(query_tiles(m[j])) * base_tiles(n[j]);
+      tile_sum += tiles[j];
+    }
+    tiles_upto = scan(tile_sum);
+    if (bad) leave_fault(g.faults, FAULT_OFFSETS);
+    if (g.groups - chunk > CHUNK) fetch(static_cast<uint64_t>(chunk) + CHUNK);
   }
 
   // Tile number t, or false when there are fewer. All lanes call and get the same answer.
@@ -241,24 +263,34 @@ struct Walk {
       if (t < tiles_before + total) break;
       tiles_before += total;
       values_before = min(values_before + __shfl_sync(0xFFFFFFFFu, values_upto, 31), uint64_t(1) << 60);
-      if (g.groups - chunk <= 32) {
+      if (g.groups - chunk <= CHUNK) {
         chunk = g.groups;  // nothing behind: later calls find nothing either
-        m = n = 0;
         tiles_upto = values_upto = 0;
         return false;
       }
-      chunk += 32;
+      chunk += CHUNK;
       load();
     }
+    // the first lane whose groups reach beyond t has it; which of its groups, every lane works out for its own
     const uint32_t who = __ffs(__ballot_sync(0xFFFFFFFFu, t < tiles_before + tiles_upto)) - 1;
-    gm = __shfl_sync(0xFFFFFFFFu, m, who), gn = __shfl_sync(0xFFFFFFFFu, n, who);
-    gq = __shfl_sync(0xFFFFFFFFu, q0, who), gb = __shfl_sync(0xFFFFFFFFu, b0, who);
-    first_value = values_before + __shfl_sync(0xFFFFFFFFu, values_upto, who) - static_cast<uint64_t>(gm) * gn;
-    qt = query_tiles(gm), bt = base_tiles(gn);
-    // queries per tile: an even split, in steps of 16 (at most TQ, so that no tile is empty)
-    width = ((qt == 1 ? gm : (gm + qt - 1) / qt) + 15) / 16 * 16;
-    last = tiles_before + __shfl_sync(0xFFFFFFFFu, tiles_upto, who);
-    first = last - static_cast<uint64_t>(qt) * bt;
+    uint64_t start = tiles_before + tiles_upto, value = values_before + values_upto;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) start -= tiles[j], value -= values[j];
+    uint32_t sq = q0[0], sb = b0[0], sm = m[0], sn = n[0];
+#pragma unroll
+    for (uint32_t j = 1; j < PER; ++j) {
+      if (t >= start + tiles[j - 1]) {
+        sq = q0[j], sb = b0[j], sm = m[j], sn = n[j];
+        start += tiles[j - 1], value += values[j - 1];
+      } else {
+        break;
+      }
+    }
+    gm = __shfl_sync(0xFFFFFFFFu, sm, who), gn = __shfl_sync(0xFFFFFFFFu, sn, who);
+    gq = __shfl_sync(0xFFFFFFFFu, sq, who), gb = __shfl_sync(0xFFFFFFFFu, sb, who);
+    first_value = __shfl_sync(0xFFFFFFFFu, value, who);
+    first = __shfl_sync(0xFFFFFFFFu, start, who);
+    split();
     return true;
   }
 };

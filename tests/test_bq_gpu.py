@@ -281,6 +281,10 @@ GROUPS = [
     ([0] * 40 + [5, 0, 300], [7] * 40 + [0, 200, 129], 130),
     (list(range(33)), list(range(33, 0, -1)), 96),
     ([2000, 0, 1], [1, 500, 40], 128),
+    ([1, 0, 3] * 43, [2, 5, 0] * 43, 32),  # 129 groups
+    ([0] * 127 + [1], [1] * 127 + [200], 48),
+    ([i % 5 for i in range(700)], [(7 * i) % 23 for i in range(700)], 96),
+    ([i % 3 * 150 for i in range(260)], [i % 4 * 100 for i in range(260)], 64),  # several tiles a group
 ]
 
 
