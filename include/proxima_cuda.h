@@ -759,9 +759,10 @@ uint32_t pxc_sq_last_fallback(const pxc_sq* h);
  * value / 2^s to e4m3, nearest, ties to even; an infinity becomes +-448 and a
  * NaN stays one.
  *
- * All entry points: 1 <= dim <= 2^20, at most 2^31 - 257 rows. The device forms
+ * All entry points: 1 <= dim <= 2^20, at most 2^31 - 1024 rows. The device forms
  * are ordered on `stream` (NULL: the context's), neither allocate nor wait and
- * may be captured into a graph; calls on one context may run concurrently. A
+ * may be captured into a graph; calls on one context may run concurrently. The
+ * context outlives the work of its calls and the graphs that hold them. A
  * failure that only the device sees (offsets that are no partition, a wait that
  * ran out) leaves that call's outputs undefined, writes nothing outside them, and is
  * reported by a later pxc_bq_* call on the context, once: PXC_CONFIGURATION

@@ -10,7 +10,7 @@
 namespace pxc {
 namespace bq {
 
-constexpr uint64_t MAX_ROWS = (uint64_t(1) << 31) - 257;  // row numbers and tile ends fit an int32
+constexpr uint64_t MAX_ROWS = (uint64_t(1) << 31) - 1024;  // row numbers and tile ends fit an int32
 constexpr uint32_t MAX_DIM = 1u << 20;
 constexpr uint64_t MAX_SIZE = uint64_t(1) << 48;  // values in an output: offsets of them cannot overflow
 
@@ -311,7 +311,7 @@ static void check_common(const pxc_ctx* ctx, uint32_t dim, int32_t dtype) {
 // Device rows are read by wide loads and tensor maps; host rows are copied, at any alignment.
 static void check_rows(const pxc_bq_rows* r, uint32_t dim, const char* name, bool device) {
   PXC_CONFIG(r != nullptr, name, 0, "null rows");
-  PXC_CONFIG(r->rows <= MAX_ROWS, name, r->rows, "at most 2^31 - 257 rows");
+  PXC_CONFIG(r->rows <= MAX_ROWS, name, r->rows, "at most 2^31 - 1024 rows");
   if (r->rows == 0) return;
   PXC_CONFIG(r->codes != nullptr && r->scales != nullptr, name, 0, "null codes or scales");
   PXC_CONFIG(!device || (reinterpret_cast<uintptr_t>(r->codes) & 15) == 0, name, reinterpret_cast<uintptr_t>(r->codes),

@@ -265,6 +265,18 @@ def test_scales_far_apart():
     assert mid.sum() >= 16 and (np.abs(got[mid] - ref[mid]) <= 2.0**-20 * ref[mid]).all()
 
 
+def test_products_take_any_scale_byte():
+    """Every pair of bytes whose product of powers stays within 32 bits, the two ends among them."""
+    codes = torch.full((255, 16), 0x38, dtype=torch.uint8, device="cuda")  # 1.0
+    scales = torch.zeros((255, 4), dtype=torch.uint8, device="cuda")
+    scales[:, 0] = torch.arange(255, device="cuda").to(torch.uint8)
+    c = BlockCodes(codes, scales, 16)
+    got = BlockQuantizer(16).product(c, c).double().cpu().numpy()
+    e = np.arange(255)[:, None] + np.arange(255)[None, :] - 254 + 4  # 16 ones
+    fits = (e >= -100) & (e <= 127)
+    assert np.array_equal(got[fits], np.exp2(e[fits].astype(np.float64)))
+
+
 # ---- grouped products ----
 def offsets(counts):
     return np.concatenate([[0], np.cumsum(counts)]).astype(np.int64)
@@ -473,6 +485,29 @@ def test_captured_graphs_replay_on_new_values():
     bq.check()
 
 
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
+    """A tile of 8,192 blocks x 224 queries takes one SM 8,192 * 4 * 112 = 3.7 M cycles at least, more than a
+    limit of 1 ms (2 M): the epilogue's wait for it ends, the kernel returns, and the next calls say so and
+    work."""
+    from proxima_b200.errors import DeviceTimeout
+    from proxima_b200.index import Context
+
+    ctx = Context(0)
+    dim = 1 << 20
+    bq = BlockQuantizer(dim, context=ctx)
+    c = BlockCodes(torch.full((224, dim), 0x38, dtype=torch.uint8, device="cuda"),
+                   torch.full((224, dim // 128), 127, dtype=torch.uint8, device="cuda"), dim)
+    assert (bq.product(c, c[:128]) == dim).all()
+    ctx.set_wait_limit(1)
+    bq.product(c, c[:128])
+    with pytest.raises(DeviceTimeout):
+        bq.check()
+    ctx.set_wait_limit(2000)
+    assert (bq.product(c, c[:128]) == dim).all()
+    bq.check()
+    ctx.close()
+
+
 def test_refusals_on_the_device():
     bq = BlockQuantizer(64)
     c = bq.encode(torch.zeros((8, 64), device="cuda"))
@@ -506,7 +541,7 @@ def test_refusals_on_the_device():
                 dict(q=R(rows.codes, rows.scales, 8, 72, 4)), dict(q=R(rows.codes, rows.scales, 8, 48, 4)),
                 dict(q=R(rows.codes, rows.scales, 8, 64, 2)), dict(q=R(rows.codes, rows.scales, 8, 64, 0)),
                 dict(q=R(None, rows.scales, 8, 64, 4)), dict(q=R(rows.codes, None, 8, 64, 4)),
-                dict(q=R(rows.codes, rows.scales, (1 << 31) - 256, 64, 4))):
+                dict(q=R(rows.codes, rows.scales, (1 << 31) - 1023, 64, 4))):
         with pytest.raises(Configuration):
             product(**bad)
     product()
