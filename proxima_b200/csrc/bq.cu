@@ -518,6 +518,16 @@ static uint64_t check_grouped(const pxc_bq_rows* q, const void* qo, const pxc_bq
   return each;
 }
 
+// `rows` rows of `width` bytes between pitches; in one piece where there is nothing between them (a 2-D copy's
+// pitch is limited).
+static void copy_rows(void* dst, uint64_t dst_pitch, const void* src, uint64_t src_pitch, uint64_t width, uint64_t rows,
+                      cudaMemcpyKind kind, cudaStream_t s) {
+  if (rows <= 1 || (dst_pitch == width && src_pitch == width))
+    PXC_CUDA(cudaMemcpyAsync(dst, src, width * rows, kind, s));
+  else
+    PXC_CUDA(cudaMemcpy2DAsync(dst, dst_pitch, src, src_pitch, width, rows, kind, s));
+}
+
 // Device copies of host rows, with the pitches that the kernels want.
 struct Staged {
   DBuf<uint8_t> codes, scales;
@@ -534,8 +544,8 @@ struct Staged {
   void load(const pxc_bq_rows& h, uint32_t dim, cudaStream_t s) {
     make(h.rows, dim);
     if (h.rows == 0) return;
-    PXC_CUDA(cudaMemcpy2DAsync(d.codes, d.ld, h.codes, h.ld, dim, h.rows, cudaMemcpyHostToDevice, s));
-    PXC_CUDA(cudaMemcpy2DAsync(d.scales, d.sld, h.scales, h.sld, blocks_of(dim), h.rows, cudaMemcpyHostToDevice, s));
+    copy_rows(d.codes, d.ld, h.codes, h.ld, dim, h.rows, cudaMemcpyHostToDevice, s);
+    copy_rows(d.scales, d.sld, h.scales, h.sld, blocks_of(dim), h.rows, cudaMemcpyHostToDevice, s);
   }
 };
 
@@ -586,10 +596,10 @@ pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint6
     x.reserve(out->rows * dim * es);
     bq::Staged c;
     c.make(out->rows, dim);
-    PXC_CUDA(cudaMemcpy2DAsync(x.p, dim * es, vectors, stride * es, dim * es, out->rows, cudaMemcpyHostToDevice, s));
+    bq::copy_rows(x.p, dim * es, vectors, stride * es, dim * es, out->rows, cudaMemcpyHostToDevice, s);
     bq::encode(ctx, x.p, dtype, dim, dim, c.d, s);
-    PXC_CUDA(cudaMemcpy2DAsync(out->codes, out->ld, c.d.codes, c.d.ld, c.d.ld, out->rows, cudaMemcpyDeviceToHost, s));
-    PXC_CUDA(cudaMemcpy2DAsync(out->scales, out->sld, c.d.scales, c.d.sld, c.d.sld, out->rows, cudaMemcpyDeviceToHost, s));
+    bq::copy_rows(out->codes, out->ld, c.d.codes, c.d.ld, c.d.ld, out->rows, cudaMemcpyDeviceToHost, s);
+    bq::copy_rows(out->scales, out->sld, c.d.scales, c.d.sld, c.d.sld, out->rows, cudaMemcpyDeviceToHost, s);
     PXC_CUDA(cudaStreamSynchronize(s));
   });
 }
@@ -624,7 +634,7 @@ pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, vo
     DBuf<uint8_t> x;
     x.reserve(rows->rows * dim * es);
     bq::decode(ctx, c.d, dim, x.p, dtype, dim, s);
-    PXC_CUDA(cudaMemcpy2DAsync(out, stride * es, x.p, dim * es, dim * es, rows->rows, cudaMemcpyDeviceToHost, s));
+    bq::copy_rows(out, stride * es, x.p, dim * es, dim * es, rows->rows, cudaMemcpyDeviceToHost, s);
     PXC_CUDA(cudaStreamSynchronize(s));
   });
 }
@@ -666,8 +676,7 @@ pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq
     groups.groups = 1;
     groups.n_each = groups.stride = base->rows;
     bq::product(ctx, q.d, b.d, dim, groups, o.p, dtype, s);
-    PXC_CUDA(cudaMemcpy2DAsync(out, stride * es, o.p, base->rows * es, base->rows * es, queries->rows,
-                               cudaMemcpyDeviceToHost, s));
+    bq::copy_rows(out, stride * es, o.p, base->rows * es, base->rows * es, queries->rows, cudaMemcpyDeviceToHost, s);
     bq::finish(ctx, s);
   });
 }

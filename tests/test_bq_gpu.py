@@ -183,7 +183,9 @@ def test_decode_takes_any_scale_byte():
 # ---- products ----
 SHAPES = [(1, 1, 1), (1, 127, 128), (1, 1000, 96), (3, 129, 64), (16, 128, 128), (17, 300, 130), (64, 64, 512),
           (65, 200, 513), (200, 333, 260), (223, 130, 640), (224, 128, 128), (225, 131, 1100), (257, 512, 768),
-          (500, 77, 2048), (700, 1111, 384), (2, 40000, 16), (4000, 5, 200), (700, 17000, 48)]
+          (500, 77, 2048), (700, 1111, 384), (2, 40000, 16), (4000, 5, 200), (700, 17000, 48),
+          # few queries over so many rows that a tile takes several times 128 of them
+          (1, 75776, 129), (3, 75000, 40), (40, 75700, 513), (60, 37800, 130)]
 
 
 @pytest.mark.parametrize("nq,n,dim", SHAPES)
