@@ -53,8 +53,14 @@ struct Items {
 
 template <class T>
 constexpr uint32_t CHUNK = 16 / sizeof(T);  // components in 16 bytes
+// Chunks of 16 bytes per lane in a block, and rows per item: 2 KB of vectors per warp in flight either way.
+// Short vectors have one chunk a lane at most, and 16 rows an item.
 template <class T>
-constexpr uint32_t WIDE_ROWS = sizeof(T) == 4 ? 4 : 8;  // 2 KB of vectors per warp in flight either way
+constexpr uint32_t FULL = 16 / CHUNK<T>;
+template <class T>
+constexpr uint32_t SHORT_DIM = 8 * CHUNK<T>;
+template <class T, uint32_t C>
+constexpr uint32_t WIDE_ROWS = C == 1 ? 16 : 16 / C;
 constexpr uint32_t NARROW_ROWS = 4;
 
 // 16 bytes of components as f32, and back.
@@ -119,12 +125,12 @@ __device__ __forceinline__ uint4 gather(const T* p) {
   }
 }
 
-template <class T, bool WIDE>
+template <class T, bool WIDE, uint32_t C>
 __global__ void __launch_bounds__(256)
     encode_kernel(const T* __restrict__ x, uint64_t stride, uint64_t rows, uint32_t dim, uint32_t blocks,
                        uint8_t* __restrict__ codes, uint64_t ld, uint8_t* __restrict__ scales, uint64_t sld,
                        uint64_t step_rows, uint32_t step_blocks) {
-  constexpr uint32_t V = CHUNK<T>, C = 16 / V, R = WIDE_ROWS<T>, U = R / 4;
+  constexpr uint32_t V = CHUNK<T>, R = WIDE_ROWS<T, C>, U = R / 4;
   const uint32_t lane = threadIdx.x & 31, l = lane & 7, group = lane >> 3;
   const uint32_t code_end = (dim + 15) / 16 * 16;
   for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
@@ -204,12 +210,12 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <class T>
+template <class T, uint32_t C>
 __global__ void __launch_bounds__(256)
     decode_wide_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales, uint64_t sld,
                        uint64_t rows, uint32_t dim, uint32_t blocks, T* __restrict__ out, uint64_t stride,
                        uint64_t step_rows, uint32_t step_blocks) {
-  constexpr uint32_t V = CHUNK<T>, C = 16 / V, R = WIDE_ROWS<T>, U = R / 4;
+  constexpr uint32_t V = CHUNK<T>, R = WIDE_ROWS<T, C>, U = R / 4;
   const uint32_t lane = threadIdx.x & 31, l = lane & 7, group = lane >> 3;
   for (Items<R> it(blocks); it.row < rows; it.next(step_rows, step_blocks, blocks)) {
     const uint32_t c0 = it.block * BLOCK + l * V;
@@ -376,8 +382,11 @@ static void encode(pxc_ctx* ctx, const void* x, int32_t dtype, uint64_t stride, 
   const uint32_t blocks = blocks_of(dim);
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const Sweep w(ctx, out.rows, blocks, WIDE_ROWS<T>, sizeof(T) == 4 ? 64 : 8);
-    auto kernel = rows_wide(x, stride, dtype) ? encode_kernel<T, true> : encode_kernel<T, false>;
+    constexpr uint32_t F = FULL<T>;
+    const bool wide = rows_wide(x, stride, dtype), few = dim <= SHORT_DIM<T>;
+    const Sweep w(ctx, out.rows, blocks, few ? WIDE_ROWS<T, 1> : WIDE_ROWS<T, F>, sizeof(T) == 4 ? 64 : 8);
+    auto kernel = few ? (wide ? encode_kernel<T, true, 1> : encode_kernel<T, false, 1>)
+                      : (wide ? encode_kernel<T, true, F> : encode_kernel<T, false, F>);
     kernel<<<w.grid, 256, 0, s>>>(static_cast<const T*>(x), stride, out.rows, dim, blocks, out.codes, out.ld,
                                   out.scales, out.sld, w.step_rows, w.step_blocks);
   });
@@ -390,9 +399,10 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
   const uint32_t blocks = blocks_of(dim);
   with_type(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const bool wide = rows_wide(out, stride, dtype);
-    const Sweep w(ctx, in.rows, blocks, wide ? WIDE_ROWS<T> : NARROW_ROWS, 64);
-    auto kernel = wide ? decode_wide_kernel<T> : decode_narrow_kernel<T>;
+    constexpr uint32_t F = FULL<T>;
+    const bool wide = rows_wide(out, stride, dtype), few = dim <= SHORT_DIM<T>;
+    const Sweep w(ctx, in.rows, blocks, !wide ? NARROW_ROWS : few ? WIDE_ROWS<T, 1> : WIDE_ROWS<T, F>, 64);
+    auto kernel = !wide ? decode_narrow_kernel<T> : few ? decode_wide_kernel<T, 1> : decode_wide_kernel<T, F>;
     kernel<<<w.grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, blocks, static_cast<T*>(out),
                                   stride, w.step_rows, w.step_blocks);
   });
