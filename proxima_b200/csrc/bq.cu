@@ -24,9 +24,9 @@ static uint32_t blocks_of(uint32_t dim) { return (dim + BLOCK - 1) / BLOCK; }
 // addresses) is done for four. Items go by a fixed step: no division stands in the loop.
 //
 // Where rows do not start on 16 bytes (an odd pitch or base), the encoder gathers the same 16 bytes from
-// narrower loads, none of which leaves them. The decoder gives a whole warp to a block then, its lanes 32
-// apart, so that each store covers neighbouring bytes: partial sectors would each be written several
-// times over.
+// narrower loads, none of which leaves them. The decoder takes short rows without gaps as one array then, and
+// else gives a whole warp to a block, its lanes 32 apart, so that each store covers neighbouring bytes: partial
+// sectors would each be written several times over.
 
 // The items of one warp: a block of the R rows from `row` on.
 template <uint32_t R>
@@ -306,6 +306,64 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Rows without gaps whose pitch is not a multiple of 16 bytes are one array all the same: a thread has 16
+// aligned bytes of it, which lie in one row or, dim >= V, in two. A chunk's codes are a funnel of the
+// words around them; it meets up to three scales.
+template <class T>
+__global__ void __launch_bounds__(256)
+    decode_flat_kernel(const uint8_t* __restrict__ codes, uint64_t ld, const uint8_t* __restrict__ scales, uint64_t sld,
+                       uint64_t rows, uint32_t dim, T* __restrict__ out, uint64_t step_rows, uint32_t step_rest) {
+  constexpr uint32_t V = CHUNK<T>, W = V / 4;
+  const uint64_t total = rows * dim, step = static_cast<uint64_t>(gridDim.x) * blockDim.x * V;
+  uint64_t at = (static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * V;
+  uint64_t row = at / dim;
+  uint32_t col = static_cast<uint32_t>(at - row * dim);
+  const uint32_t last_word = (dim - 1) / 4;
+  for (; at < total; at += step) {
+    const uint8_t* s = scales + row * sld;
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(codes + row * ld);
+    const bool next = row + 1 < rows;  // where not, what lies behind is not stored
+    const uint32_t* c2 = next ? reinterpret_cast<const uint32_t*>(codes + (row + 1) * ld) : c;
+    const uint32_t split = min(V, dim - col), cut = min(split, BLOCK - (col & (BLOCK - 1)));
+    uint32_t w[W + 1], w2[W];
+#pragma unroll
+    for (uint32_t i = 0; i <= W; ++i) w[i] = __ldg(c + min(col / 4 + i, last_word));
+    if (split < V) {
+#pragma unroll
+      for (uint32_t i = 0; i < W; ++i) w2[i] = __ldg(c2 + i);
+    }
+    const float f0 = scale_value(s[col / BLOCK]);
+    const float f1 = cut < split ? scale_value(s[col / BLOCK + 1]) : f0;
+    const float f2 = split < V ? scale_value(next ? s[sld] : s[0]) : f1;
+    uint64_t q = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < W; ++i)
+      q |= static_cast<uint64_t>(__funnelshift_r(w[i], w[i + 1], 8 * (col & 3))) << (32 * i);
+    if (split < V) {
+      uint64_t behind = w2[0];
+      if constexpr (W == 2) behind |= static_cast<uint64_t>(w2[1]) << 32;
+      q = (q & ((uint64_t(1) << (8 * split)) - 1)) | behind << (8 * split);
+    }
+    float v[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; i += 2) {
+      const float2 two = from_codes(static_cast<uint32_t>(q >> (8 * i)) & 0xFFFFu);
+      v[i] = two.x * (i < cut ? f0 : i < split ? f1 : f2);
+      v[i + 1] = two.y * (i + 1 < cut ? f0 : i + 1 < split ? f1 : f2);
+    }
+    if (at + V <= total) {
+      __stcs(reinterpret_cast<uint4*>(out + at), pack<T>(v));
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < V - 1; ++i)
+        if (at + i < total) out[at + i] = from_f32<T>(v[i]);
+    }
+    row += step_rows;
+    col += step_rest;
+    if (col >= dim) col -= dim, ++row;
+  }
+}
+
 // ---- host ----
 static void check_common(const pxc_ctx* ctx, uint32_t dim, int32_t dtype) {
   PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
@@ -401,6 +459,17 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr uint32_t F = FULL<T>;
     const bool wide = rows_wide(out, stride, dtype), few = dim <= SHORT_DIM<T>;
+    // Short rows leave the narrow kernel's warps part empty (1M x 31 f32: 92 us, as one array 42 us); long ones
+    // suit it (100003 x 1001 bf16: 75 us, as one array 79 us).
+    if (!wide && stride == dim && dim >= CHUNK<T> && blocks <= 2 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+      const uint64_t threads = (in.rows * dim + CHUNK<T> - 1) / CHUNK<T>;
+      const unsigned grid =
+          static_cast<unsigned>(std::min<uint64_t>((threads + 255) / 256, static_cast<uint64_t>(ctx->sm_count) * 32));
+      const uint64_t step = static_cast<uint64_t>(grid) * 256 * CHUNK<T>;
+      decode_flat_kernel<T><<<grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, static_cast<T*>(out),
+                                                 step / dim, static_cast<uint32_t>(step % dim));
+      return;
+    }
     const Sweep w(ctx, in.rows, blocks, !wide ? NARROW_ROWS : few ? WIDE_ROWS<T, 1> : WIDE_ROWS<T, F>, 64);
     auto kernel = !wide ? decode_narrow_kernel<T> : few ? decode_wide_kernel<T, 1> : decode_wide_kernel<T, F>;
     kernel<<<w.grid, 256, 0, s>>>(in.codes, in.ld, in.scales, in.sld, in.rows, dim, blocks, static_cast<T*>(out),

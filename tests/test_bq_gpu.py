@@ -119,7 +119,7 @@ def special_rows(dim, seed, dtype):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("dim", [1, 15, 16, 17, 96, 127, 128, 129, 300, 768, 1001, 4096])
+@pytest.mark.parametrize("dim", [1, 7, 9, 15, 16, 17, 31, 96, 127, 128, 129, 131, 250, 257, 300, 768, 1001, 4096])
 def test_encode_and_decode_are_the_definition(dim, kind):
     dtype = DTYPES[kind]
     x = special_rows(dim, dim, dtype)
