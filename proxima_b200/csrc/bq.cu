@@ -488,6 +488,32 @@ static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, uint64_t sms) {
   return 1;
 }
 
+// The tile of a dense product: `width` queries, by 128 rows or as a pair by 256.
+struct Shape {
+  uint32_t width;
+  bool pair;
+};
+// The one whose rounds over the SMs take least (200 x 2000 x 128: 8.6 us with the widest tiles, 6.4 so; 1024 x 1024 x
+// 1024: 11.5, 9.7). The widest even split is always among those looked at. A block of a tile takes 340 cycles and 1.4 a query (measured from
+// 128 to 224 queries a tile), a tile itself some 1,400, and a CTA on its own a twelfth longer than as one of a pair.
+static Shape dense_shape(uint64_t nq, uint64_t rows, uint32_t kblocks, uint64_t sms) {
+  Shape best{};
+  uint64_t least = ~uint64_t(0);
+  for (uint32_t width = bq_tc::MAX_Q; width >= 16; width -= 16) {
+    const uint64_t qt = (nq + width - 1) / width;
+    if (up((nq + qt - 1) / qt, 16) != width) continue;  // the even split is another width
+    if (qt > 1 && width < 64) break;  // the rows would pass too often (100 x 2000 x 2048: 11.5 us, by 16 at a time 13)
+    for (int pair = 0; pair < 2; ++pair) {
+      if (pair && (width <= 112 || rows <= bq_tc::BM)) continue;
+      const uint64_t tall = bq_tc::BM << pair, slots = sms >> pair;
+      const uint64_t rounds = (qt * ((rows + tall - 1) / tall) + slots - 1) / slots;
+      const uint64_t cost = rounds * (static_cast<uint64_t>(kblocks) * (240 + width) + 1000) * (pair ? 12 : 13);
+      if (cost < least) least = cost, best = Shape{width, pair != 0};
+    }
+  }
+  return best;
+}
+
 static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, const Groups& g, void* out,
                     int32_t dtype, cudaStream_t s) {
   using namespace bq_tc;
@@ -503,16 +529,21 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   p.out = out;
   p.dim = dim;
   p.kblocks = blocks_of(dim);
-  // The widest tile: dense, the walk's even split; grouped, room for twice the mean, so that most groups
-  // are one tile and the rings stay deep.
   const bool dense = !g.q_offsets;
-  const uint64_t mean = q.rows / g.groups;
-  p.tile_q = dense ? MAX_Q : static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, std::max<uint64_t>(32, up(2 * mean, 32))));
-  const uint64_t qt = (q.rows + MAX_Q - 1) / MAX_Q;
-  p.q_rows = dense ? static_cast<uint32_t>(up((q.rows + qt - 1) / qt, 16)) : p.tile_q;
-  // Pairs where there are enough queries to be bound by the matrix instructions and what feeds them.
-  const bool pair = p.q_rows > 112 && (dense ? b.rows > BM : mean > 112);
-  p.subs = dense && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
+  bool pair;
+  if (dense) {
+    const Shape shape = dense_shape(q.rows, b.rows, p.kblocks, ctx->sm_count);
+    p.tile_q = p.q_rows = shape.width;
+    pair = shape.pair;
+    p.subs = q.rows <= shape.width && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
+  } else {
+    // room for twice the mean, so that most groups are one tile and the rings stay deep; pairs where the mean
+    // fills them (8192 queries over 32 groups: 45 us, without 46; over 500 lists of 40: 47 us, without 44)
+    const uint64_t mean = q.rows / g.groups;
+    p.tile_q = p.q_rows = static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, std::max<uint64_t>(32, up(2 * mean, 32))));
+    pair = mean > 112;
+    p.subs = 1;
+  }
   const uint32_t tile_rows = pair ? 2 * BM : p.subs * BM;
   p.tile_log2 = tile_rows == BM ? 7 : tile_rows == 2 * BM ? 8 : 9;
   p.q_load = pair ? p.q_rows / 2 : p.q_rows;
@@ -530,7 +561,7 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
   // no more CTAs than tiles, where the host can tell
   uint64_t tiles = ctx->sm_count;
   if (dense)
-    tiles = qt * ((b.rows + tile_rows - 1) / tile_rows);
+    tiles = (q.rows + p.tile_q - 1) / p.tile_q * ((b.rows + tile_rows - 1) / tile_rows);
   else if (!g.b_offsets)
     tiles = (std::min<uint64_t>(g.groups, q.rows) + q.rows / p.tile_q) * ((g.n_each + tile_rows - 1) / tile_rows);
   const uint32_t ctas = pair ? 2 : 1;
