@@ -488,9 +488,9 @@ def test_captured_graphs_replay_on_new_values():
 
 
 def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
-    """A tile of 8,192 blocks x 224 queries takes one SM 8,192 * 4 * 112 = 3.7 M cycles at least, more than a
-    limit of 1 ms (2 M): the epilogue's wait for it ends, the kernel returns, and the next calls say so and
-    work."""
+    """One group of 224 queries is one tile; its 8,192 blocks take 8,192 * 4 * 112 = 3.7 M cycles at least, more
+    than a limit of 1 ms (2 M): the epilogue's wait for it ends, the kernel returns, and the next calls
+    say so and work."""
     from proxima_b200.errors import DeviceTimeout
     from proxima_b200.index import Context
 
@@ -499,12 +499,14 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable():
     bq = BlockQuantizer(dim, context=ctx)
     c = BlockCodes(torch.full((224, dim), 0x38, dtype=torch.uint8, device="cuda"),
                    torch.full((224, dim // 128), 127, dtype=torch.uint8, device="cuda"), dim)
-    assert (bq.product(c, c[:128]) == dim).all()
+    off = torch.tensor([0, 224], device="cuda")
+    assert (bq.grouped_product(c, off, c[:128]) == dim).all()
     ctx.set_wait_limit(1)
-    bq.product(c, c[:128])
+    bq.grouped_product(c, off, c[:128])
     with pytest.raises(DeviceTimeout):
         bq.check()
     ctx.set_wait_limit(2000)
+    assert (bq.grouped_product(c, off, c[:128]) == dim).all()
     assert (bq.product(c, c[:128]) == dim).all()
     bq.check()
     ctx.close()
