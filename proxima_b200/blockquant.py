@@ -74,7 +74,7 @@ def _torch() -> _Torch:
     return _torch_parts
 
 
-@dataclass
+@dataclass(slots=True)
 class BlockCodes:
     """Encoded rows: ``codes`` (n, dim rounded up to 16) and ``scales`` (n, blocks rounded up
     to 4), both uint8, tensors or arrays. Row slices are views."""
@@ -100,14 +100,17 @@ class BlockQuantizer:
     """Encodes, decodes and multiplies rows of ``dim`` components (``pxc_bq_*``)."""
 
     def __init__(self, dim: int, context=None):
-        from .index import Context
-
-        if not 1 <= int(dim) <= 1 << 20:
+        dim = int(dim)
+        if not 1 <= dim <= 1 << 20:
             raise Configuration("dim", dim, "must be between 1 and 1048576")
-        self.dim = int(dim)
-        self.blocks = -(-self.dim // BLOCK)
-        self.ctx = context or Context.default()
-        self._ld, self._sld = _up(self.dim, 16), _up(self.blocks, 4)
+        if context is None:
+            from .index import Context
+
+            context = Context.default()
+        self.dim = dim
+        self.ctx = context
+        self.blocks = -(-dim // BLOCK)
+        self._ld, self._sld = (dim + 15) & ~15, (self.blocks + 3) & ~3
 
     # -- arguments --
     def _stream(self, tensor) -> int:
@@ -149,6 +152,8 @@ class BlockQuantizer:
         """(n, dim), an array in one of the types."""
         if _is_cuda(vectors):
             v = vectors
+            if v.ndim == 2 and v.shape[1] == self.dim:
+                return v
         else:
             v = np.asarray(vectors)
             if v.dtype not in (np.float32, np.float16):
@@ -164,20 +169,22 @@ class BlockQuantizer:
         """Each row's codes and scales. Rows of a tensor may be strided. An infinity becomes the
         largest code of its block, 448 times the scale; a NaN stays one."""
         v = self._vectors(vectors)
-        n, ld, sld = v.shape[0], self._ld, self._sld
+        n, dim, ld, sld = len(v), self.dim, self._ld, self._sld
         if _is_cuda(v):
             t = _torch()
-            code = _dtype_code(v.dtype)
+            code = _codes.get(v.dtype)
+            if code is None:
+                code = _dtype_code(v.dtype)
             stream = self._stream(v)
             row, step = v.stride()
-            if (self.dim > 1 and step != 1) or (n > 1 and row < self.dim):
+            if (step != 1 and dim > 1) or (row < dim and n > 1):
                 v = v.contiguous()
-                row = self.dim
+                row = dim
             codes = t.empty(n, ld, dtype=t.uint8, device=v.device)
             scales = codes.new_empty(n, sld)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
-            t.encode(self.ctx.handle, v.data_ptr(), code, row if n > 1 else self.dim, self.dim, C.byref(rows), stream)
-            return BlockCodes(codes, scales, self.dim)
+            t.encode(self.ctx.handle, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
+            return BlockCodes(codes, scales, dim)
         v = np.ascontiguousarray(v)
         codes, scales = np.zeros((n, ld), np.uint8), np.zeros((n, sld), np.uint8)
         rows = N.PxcBqRows(N.ptr(codes), N.ptr(scales), n, ld, sld)
