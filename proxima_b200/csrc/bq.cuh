@@ -127,7 +127,10 @@ struct Walk {
   uint32_t qt = 0, bt = 0, width = 0;
 
   __device__ __forceinline__ Walk(const Groups& groups, uint32_t lane_id, uint32_t queries, uint32_t rows_log2)
-      : g(groups), lane(lane_id), TQ(queries), tb_log2(rows_log2) {
+      : g(groups), lane(lane_id), TQ(queries), tb_log2(rows_log2) {}
+
+  // Reads the first chunk; before find().
+  __device__ __forceinline__ void start() {
     if (g.q_offsets) {
       fetch(0);
       load();

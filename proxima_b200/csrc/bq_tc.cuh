@@ -339,6 +339,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t rank = PAIR ? blockIdx.x & 1 : 0;  // in the cluster: 0 leads
 
   if (warp == 1) tmem_alloc<G>(&c.tmem);
+  Walk walk(p.groups, lane, p.tile_q, p.tile_log2);
+  if (warp == 3) walk.start();  // the offsets are on their way while the others set up
   if (threadIdx.x == 0) {
     c.failed = 0;
     for (uint32_t s = 0; s < p.stages; ++s) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
@@ -515,7 +517,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     asm volatile("cp.async.wait_all;" ::: "memory");  // landed before the CTA exits
   } else if (warp == 3) {
     // ---- the walk over tiles: the same in both CTAs of a pair ----
-    Walk walk(p.groups, lane, p.tile_q, p.tile_log2);
     Ring s;
     for (uint64_t k = blockIdx.x / G;; k += gridDim.x / G) {
       const bool any = walk.find(k, t);
