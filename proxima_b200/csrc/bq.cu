@@ -494,8 +494,9 @@ struct Shape {
   bool pair;
 };
 // The one whose rounds over the SMs take least (200 x 2000 x 128: 8.6 us with the widest tiles, 6.4 so; 1024 x 1024 x
-// 1024: 11.5, 9.7). The widest even split is always among those looked at. A block of a tile takes 340 cycles and 1.4 a query (measured from
-// 128 to 224 queries a tile), a tile itself some 1,400, and a CTA on its own a twelfth longer than as one of a pair.
+// 1024: 11.5, 9.7). The widest even split is always among those looked at. A block of a tile takes 340 cycles and 1.4 a
+// query (measured from 128 to 224 queries a tile), a tile itself some 1,400, and a CTA on its own a twelfth longer than
+// as one of a pair.
 static Shape dense_shape(uint64_t nq, uint64_t rows, uint32_t kblocks, uint64_t sms) {
   Shape best{};
   uint64_t least = ~uint64_t(0);

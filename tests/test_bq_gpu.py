@@ -299,7 +299,7 @@ GROUPS = [
     ([0] * 127 + [1], [1] * 127 + [200], 48),
     ([i % 5 for i in range(700)], [(7 * i) % 23 for i in range(700)], 96),
     ([i % 3 * 150 for i in range(260)], [i % 4 * 100 for i in range(260)], 64),  # several tiles a group
-    # groups of so many rows that a tile takes several times 128 of them
+    # many long lists under few queries, some of them without any
     ([i % 5 * 20 for i in range(80)], [1500 + 77 * (i % 40) for i in range(80)], 130),
     ([i % 4 for i in range(120)], [1500 + 177 * (i % 20) for i in range(120)], 96),
 ]
