@@ -34,8 +34,10 @@
 //
 // A scale slot, in shared memory or TMEM, is written again only after the MMAs that read it have
 // completed (sf_empty), so nothing hangs on the order of copies and MMAs beyond the documented one.
-// Every wait is bounded; when one runs out the CTA leaves FAULT_TIMEOUT, drains its copies and
-// MMAs, frees TMEM and returns.
+// Every wait is bounded. When one runs out, the CTA (of a pair: both) stops, waits for its copies and
+// MMAs in flight, leaves FAULT_TIMEOUT, frees TMEM and returns. Both CTAs of a pair count their copies
+// on the leader's barriers, and after a failure they may have stopped at different stages: the
+// leader makes up the share of each stage that never comes and waits for the one that does (drain()).
 #pragma once
 #include "bq.cuh"
 #include "sm100.cuh"
@@ -60,6 +62,9 @@ constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TILE_SLOTS = 16;  // more than stages, so that the walk never holds the loads of short tiles back
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
 constexpr uint32_t MAX_STAGES = 12;
+// For copies and MMAs in flight, which end by themselves: not the caller's limit, or a short one would
+// let a CTA go before them.
+constexpr uint64_t DRAIN_CYCLES = 2000000000;
 
 struct TileSlot {
   Tile tile;
@@ -96,6 +101,8 @@ struct Control {
   uint64_t done;
   uint32_t tmem;
   volatile uint32_t failed;
+  uint32_t peer_failed;  // of a pair: the cluster address of the other CTA's `failed`
+  uint32_t issued, loaded[MAX_STAGES];  // stages that the producer filled, and the bytes of each slot's last
 };
 
 __host__ __device__ inline uint32_t q_atoms(const Params& p) { return (p.q_rows + 127) / 128; }
@@ -204,6 +211,23 @@ __device__ __forceinline__ void arrive_relaxed(uint64_t* bar) {
 __device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ uint32_t in_peer(const volatile void* here, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(a)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(const_cast<const void*>(here)))), "r"(rank ^ 1));
+  return a;
+}
+__device__ __forceinline__ uint32_t load_cluster(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+// Bytes that no copy will bring, counted as arrived.
+__device__ __forceinline__ void complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(sm100::smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -235,10 +259,16 @@ __device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
     return ok != 0;
   }
 }
+// Stops this CTA's roles at their next late wait, and the other CTA's of a pair.
+template <bool PAIR>
+__device__ __forceinline__ void fail(Control& c) {
+  c.failed = 1;
+  if constexpr (PAIR) asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], 1;" ::"r"(c.peer_failed) : "memory");
+}
 // A bounded wait of one thread: a ready barrier costs one test, and only a late one looks at the
 // clock and at the CTA's failure flag. Waits are made by one lane: tests by all 32 take turns
 // in the shared-memory pipe and cost every role of the CTA some 200 cycles each.
-template <bool PEER = false>
+template <bool PAIR, bool PEER = false>
 __device__ __forceinline__ bool wait_one(Control& c, uint64_t* bar, uint32_t parity, uint64_t limit) {
   if (try_wait<PEER>(bar, parity)) return true;
   const uint64_t start = clock64();
@@ -246,21 +276,40 @@ __device__ __forceinline__ bool wait_one(Control& c, uint64_t* bar, uint32_t par
     if (try_wait<PEER>(bar, parity)) return true;
     if (c.failed) return false;
     if (clock64() - start > limit) {
-      c.failed = 1;
+      fail<PAIR>(c);
       return false;
     }
   }
 }
 // The same for a whole warp.
+template <bool PAIR>
 __device__ __forceinline__ bool wait_warp(Control& c, uint64_t* bar, uint32_t parity, uint64_t limit) {
   bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = wait_one(c, bar, parity, limit);
+  if ((threadIdx.x & 31) == 0) ok = wait_one<PAIR>(c, bar, parity, limit);
   return __shfl_sync(0xFFFFFFFFu, ok, 0);
 }
-// Before the CTA ends: regardless of failures, as long as the limit lasts.
-__device__ __forceinline__ void wait_drained(uint64_t* bar, uint32_t parity, uint64_t limit) {
+// Before the CTA ends, regardless of failures: for what is in flight, at the latest DRAIN_CYCLES after `start`.
+__device__ __forceinline__ void wait_drained(uint64_t* bar, uint32_t parity, uint64_t start) {
+  while (!try_wait<false>(bar, parity) && clock64() - start <= DRAIN_CYCLES) {
+  }
+}
+// After a failure, by one thread of the CTA (of a pair: of the leader, once both CTAs' roles have ended): waits
+// until every copy that was issued has landed. The last use of each slot, oldest first; earlier ones have been waited
+// for, since a slot is filled again only after its MMAs. Of a pair, either producer may be up to a
+// ring ahead of the other. Where only the leader filled a stage, the half that it expects of
+// the other is made up; where only the other did, its half alone is expected.
+template <bool PAIR>
+__device__ __forceinline__ void drain(Control& c, uint32_t stages) {
   const uint64_t start = clock64();
-  while (!try_wait<false>(bar, parity) && clock64() - start <= limit) {
+  const uint32_t mine = c.issued, theirs = PAIR ? load_cluster(in_peer(&c.issued, 0)) : mine;
+  const uint32_t most = max(mine, theirs);
+  for (uint32_t j = most > stages ? most - stages : 0; j < most; ++j) {
+    const uint32_t i = j % stages;
+    if (PAIR && j >= theirs)
+      complete_tx(&c.full[i], c.loaded[i]);
+    else if (PAIR && j >= mine)
+      sm100::mbar_arrive_expect_tx(&c.full[i], load_cluster(in_peer(&c.loaded[i], 0)));
+    wait_drained(&c.full[i], (j / stages) & 1, start);
   }
 }
 
@@ -283,12 +332,13 @@ struct Ring {
 
 // The next tile of the ring for one of its readers, a thread or a warp. False at the end or after
 // a failure.
+template <bool PAIR>
 struct Reader {
   Control& c;
   const uint64_t limit;
   Ring at = {};
   __device__ __forceinline__ bool next_one(Tile& t) {
-    if (!wait_one(c, &c.tile_full[at.i], at.ph, limit)) return false;
+    if (!wait_one<PAIR>(c, &c.tile_full[at.i], at.ph, limit)) return false;
     const bool any = c.tiles[at.i].valid != 0;
     t = c.tiles[at.i].tile;
     sm100::mbar_arrive(&c.tile_empty[at.i]);
@@ -296,7 +346,7 @@ struct Reader {
     return any;
   }
   __device__ __forceinline__ bool next_warp(Tile& t) {
-    if (!wait_warp(c, &c.tile_full[at.i], at.ph, limit)) return false;
+    if (!wait_warp<PAIR>(c, &c.tile_full[at.i], at.ph, limit)) return false;
     const bool any = c.tiles[at.i].valid != 0;
     t = c.tiles[at.i].tile;
     __syncwarp();
@@ -343,6 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 3) walk.start();  // the offsets are on their way while the others set up
   if (threadIdx.x == 0) {
     c.failed = 0;
+    if constexpr (PAIR) c.peer_failed = in_peer(&c.failed, rank);
     for (uint32_t s = 0; s < p.stages; ++s) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
     for (uint32_t s = 0; s < p.sf_slots; ++s)
       mbar_init(&c.sf_full[s], 32), mbar_init(&c.sf_peer[s], 1), mbar_init(&c.sf_empty[s], 1);
@@ -360,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = c.tmem;
   const uint64_t limit = p.wait_cycles;
-  Reader reader{c, limit};
+  Reader<PAIR> reader{c, limit};
   Tile t;
 
   if (warp == 0) {
@@ -372,16 +423,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       while (ok && reader.next_one(t)) {
         const uint32_t width = round16(t.queries), load = width / G;
         const uint32_t boxes = (load + p.q_box - 1) / p.q_box;
-        const uint32_t bytes = G * (subs * BASE_BYTES + boxes * p.q_box * KB);
+        const uint32_t bytes = subs * BASE_BYTES + boxes * p.q_box * KB;  // this CTA's
         const int32_t b0 = t.b0 + rank * BM, q0 = t.q0 + rank * load;
         for (uint32_t kb = 0; kb < kblocks; ++kb) {
-          if (!(ok = wait_one(c, &c.empty[s.i], s.ph ^ 1, limit))) break;
+          if (!(ok = wait_one<PAIR>(c, &c.empty[s.i], s.ph ^ 1, limit))) break;
           unsigned char* dst = smem + static_cast<size_t>(s.i) * per_stage;
           unsigned char* dst_q = dst + subs * BASE_BYTES;
           if constexpr (PAIR) {
             // both CTAs' bytes are counted on the leader's barrier
             const uint32_t bar = leaders(&c.full[s.i]);
-            if (rank == 0) mbar_arrive_expect_tx(&c.full[s.i], bytes);
+            if (rank == 0) mbar_arrive_expect_tx(&c.full[s.i], G * bytes);
             tma_load_pair(dst, &map_b, bar, kb * KB, b0);
             for (uint32_t i = 0; i < boxes; ++i)
               tma_load_pair(dst_q + i * p.q_box * KB, &map_q, bar, kb * KB, q0 + i * p.q_box);
@@ -392,15 +443,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (uint32_t i = 0; i < boxes; ++i)
               tma_load_2d(dst_q + i * p.q_box * KB, &map_q, &c.full[s.i], kb * KB, q0 + i * p.q_box);
           }
+          c.loaded[s.i] = bytes;
           ++issued;
           s.step(p.stages);
         }
       }
-      // every copy has landed before the CTA (of a pair: the leader, and with it the other) exits: the
-      // last use of each stage, oldest first
-      if (rank == 0)
-        for (uint32_t j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
-          wait_drained(&c.full[j % p.stages], (j / p.stages) & 1, limit);
+      c.issued = issued;
     }
   } else if (warp == 1 && rank == 0) {
     // ---- MMA ----
@@ -415,18 +463,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t last_steps = (p.dim - (kblocks - 1) * KB + MMA_K - 1) / MMA_K;
       while (ok && reader.next_one(t)) {
         const uint32_t width = round16(t.queries);
-        if (!(ok = wait_one<PAIR>(c, &c.acc_empty[acc.i], acc.ph ^ 1, limit))) break;
+        if (!(ok = wait_one<PAIR, PAIR>(c, &c.acc_empty[acc.i], acc.ph ^ 1, limit))) break;
         tc_fence_after();
         const uint32_t d = tmem + acc.i * p.acc_cols, idesc0 = idesc_mxf8(G * BM, width, 0);
         for (uint32_t kb = 0; kb < kblocks; ++kb) {
           const uint32_t sfa = tmem + p.sf_col + (quad % SF_TMEM) * p.sf_cols, sfb = sfa + 4 * subs;
           if ((kb & 3) == 0) {
-            if (!(ok = wait_one(c, &c.sf_full[sf.i], sf.ph, limit))) break;
+            if (!(ok = wait_one<PAIR>(c, &c.sf_full[sf.i], sf.ph, limit))) break;
             if constexpr (PAIR)
-              if (!(ok = wait_one<true>(c, &c.sf_peer[sf.i], sf.ph, limit))) break;
+              if (!(ok = wait_one<PAIR, true>(c, &c.sf_peer[sf.i], sf.ph, limit))) break;
             if (p.sf_slots > SF_TMEM && quad >= SF_TMEM) {
               // the words in the same TMEM columns before are done with
-              if (!(ok = wait_one(c, &c.sf_empty[old.i], old.ph, limit))) break;
+              if (!(ok = wait_one<PAIR>(c, &c.sf_empty[old.i], old.ph, limit))) break;
               old.step(p.sf_slots);
             }
             fence_proxy_async();  // the words came by generic copies
@@ -437,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             copy_scales<G>(sfb, from + subs * ATOM);
             if (width > 128) copy_scales<G>(sfb + 4, from + (subs + 1) * ATOM);
           }
-          if (!ready && !(ok = wait_one(c, &c.full[s.i], s.ph, limit))) break;
+          if (!ready && !(ok = wait_one<PAIR>(c, &c.full[s.i], s.ph, limit))) break;
           tc_fence_after();
           // look at the next stage now: the answer is there once these MMAs are issued
           Ring following = s;
@@ -469,7 +517,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // all MMAs complete before TMEM is released
       commit<G>(&c.done);
-      wait_drained(&c.done, 0, limit);
+      wait_drained(&c.done, 0, clock64());
     }
   } else if (PAIR && warp == 1) {
     // ---- the second CTA of a pair: tells the leader of its scale words ----
@@ -478,14 +526,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       while (ok && reader.next_one(t)) {
         for (uint32_t w = 0; w < (kblocks + 3) / 4; ++w) {
-          if (!(ok = wait_one(c, &c.sf_full[sf.i], sf.ph, limit))) break;
+          if (!(ok = wait_one<PAIR>(c, &c.sf_full[sf.i], sf.ph, limit))) break;
           fence_proxy_async();
           arrive_cluster(leaders(&c.sf_peer[sf.i]));
           sf.step(p.sf_slots);
         }
       }
-      // the leader's signals to this CTA are on their way until its last one is here
-      wait_drained(&c.done, 0, limit);
     }
   } else if (warp == 2) {
     // ---- scales ----
@@ -495,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t words = (kblocks + 3) / 4, columns = (t.queries + 31) / 32;
       const uint64_t b0 = static_cast<uint64_t>(t.b0) + rank * BM;
       for (uint32_t w = 0; w < words; ++w) {
-        if (!(ok = wait_warp(c, &c.sf_empty[sf.i], sf.ph ^ 1, limit))) break;
+        if (!(ok = wait_warp<PAIR>(c, &c.sf_empty[sf.i], sf.ph ^ 1, limit))) break;
         const uint32_t to = smem_u32(sf_ring) + sf.i * per_sf + lane * 16;
         for (uint32_t i = 0; i < subs; ++i) {
 #pragma unroll
@@ -520,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     Ring s;
     for (uint64_t k = blockIdx.x / G;; k += gridDim.x / G) {
       const bool any = walk.find(k, t);
-      if (!wait_warp(c, &c.tile_empty[s.i], s.ph ^ 1, limit)) break;
+      if (!wait_warp<PAIR>(c, &c.tile_empty[s.i], s.ph ^ 1, limit)) break;
       if (lane == 0) {
         c.tiles[s.i].tile = t;
         c.tiles[s.i].valid = any;
@@ -535,7 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     T* out = static_cast<T*>(p.out);
     Ring acc;
     while (reader.next_warp(t)) {
-      if (!wait_warp(c, &c.acc_full[acc.i], acc.ph, limit)) break;
+      if (!wait_warp<PAIR>(c, &c.acc_full[acc.i], acc.ph, limit)) break;
       tc_fence_after();
       // Outputs are stored with the streaming hint: without it a large one drives the operands out of L2
       // (4096 x 65536 x 768 f32: 337 us, with it 290).
@@ -587,7 +633,18 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();  // neither CTA goes while the other may read or signal it
+  if constexpr (PAIR) cluster_sync();  // both have issued all that they will, and `failed` is the same in both
+  // without a failure the MMAs waited for every copy
+  if (c.failed) {
+    if (rank == 0 && threadIdx.x == 0) drain<PAIR>(c, p.stages);
+    __syncwarp();
+    if constexpr (PAIR) cluster_sync();  // neither CTA goes while copies into it or signals of it are in flight
+  }
+  // the leader's signals to the other CTA are on their way until its last one is here
+  if (PAIR && rank != 0 && warp == 1) {
+    if (lane == 0) wait_drained(&c.done, 0, clock64());
+    __syncwarp();
+  }
   tc_fence_after();
   if (warp == 1) tmem_free<G>(tmem);
   if (threadIdx.x == 0 && c.failed) leave_fault(p.groups.faults, FAULT_TIMEOUT);
