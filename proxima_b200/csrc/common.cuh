@@ -170,12 +170,13 @@ struct pxc_ctx {
 };
 
 namespace pxc {
-// RAII device selection.
+// RAII device selection. A thread's first CUDA call may be a driver one (the encoding of a tensor map), which wants
+// the device's context bound to the thread: naming the device binds it, even where it is the current one already.
 struct DeviceGuard {
   int prev = -1;
   explicit DeviceGuard(int dev) {
     cudaGetDevice(&prev);
-    if (prev != dev) PXC_CUDA(cudaSetDevice(dev));
+    PXC_CUDA(cudaSetDevice(dev));
   }
   ~DeviceGuard() {
     int cur = -1;

@@ -1,0 +1,53 @@
+"""Ways of calling the block quantiser that the documentation allows."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+from proxima_b200 import _native as N
+from proxima_b200.blockquant import BlockCodes, BlockQuantizer
+from proxima_b200.errors import Configuration
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def codes_of(bq, rows, seed):
+    """Small integers: products of them are exact in any order."""
+    g = torch.Generator().manual_seed(seed)
+    return bq.encode(torch.randint(-3, 4, (rows, bq.dim), generator=g).float().cuda())
+
+
+def in_a_thread(call):
+    """What `call` returns in a thread that has made no CUDA call before."""
+    got = []
+
+    def work():
+        try:
+            got.append(call())
+        except BaseException as e:
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    if isinstance(got[0], BaseException):
+        raise got[0]
+    return got[0]
+
+
+def test_a_products_thread_needs_no_cuda_call_before():
+    bq = BlockQuantizer(48)
+    q, b = codes_of(bq, 20, 1), codes_of(bq, 40, 2)
+    off = torch.tensor([0, 7, 20], device="cuda")
+    want, parts = bq.product(q, b), bq.grouped_product(q, off, b)
+    out = torch.empty((20, 40), device="cuda")
+    torch.cuda.synchronize()
+    in_a_thread(lambda: bq.product(q, b, out=out))
+    assert torch.equal(out, want)
+    assert torch.equal(in_a_thread(lambda: bq.product(q, b)), want)
+    assert torch.equal(in_a_thread(lambda: bq.grouped_product(q, off, b)), parts)
+    assert torch.equal(in_a_thread(lambda: bq.encode(bq.decode(q))).codes, q.codes)
+    h = BlockCodes(q.codes.cpu().numpy(), q.scales.cpu().numpy(), 48)
+    assert np.array_equal(in_a_thread(lambda: bq.product(h, h)), bq.product(q, q).cpu().numpy())
