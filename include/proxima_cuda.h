@@ -765,8 +765,15 @@ uint32_t pxc_sq_last_fallback(const pxc_sq* h);
  * context outlives the work of its calls and the graphs that hold them. A
  * failure that only the device sees (offsets that are no partition, a wait that
  * ran out) leaves that call's outputs undefined, writes nothing outside them, and is
- * reported by a later pxc_bq_* call on the context, once: PXC_CONFIGURATION
- * ("offsets") or PXC_TIMEOUT. The host forms report their own. */
+ * reported once, as PXC_CONFIGURATION ("offsets") or PXC_TIMEOUT, to its own caller
+ * and to no other:
+ *   - a host form reports its own failure, and nobody else's;
+ *   - one of a session's call is reported by a later call of that session;
+ *   - one of a device form called with the context itself is reported by a
+ *     later such call, or pxc_bq_check, on the same stream; if it was
+ *     captured into a graph, on any stream.
+ * So callers that share a context and a stream, and run beside one another, take a
+ * session each. */
 #define PXC_DTYPE_F32 0
 #define PXC_DTYPE_F16 1
 #define PXC_DTYPE_BF16 2
@@ -822,8 +829,31 @@ pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_quer
                                          uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
                                          pxc_error* err);
 /* Waits for `stream` (NULL: the context's) and reports a failure that the device
- * forms left, as above. */
+ * forms called with the context itself left, as above. */
 pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err);
+
+/* A caller's session: the device forms above, with failures of their own. Creating
+ * one may allocate; calls of one session may run concurrently. It may go before
+ * its work has run, whose failures nobody is told of then, or after the context. */
+typedef struct pxc_bq_session pxc_bq_session;
+pxc_status pxc_bq_session_create(pxc_ctx* ctx, pxc_bq_session** out, pxc_error* err);
+void pxc_bq_session_destroy(pxc_bq_session* session);
+pxc_status pxc_bq_session_encode(pxc_bq_session* session, const void* d_vectors, int32_t dtype, uint64_t stride,
+                                 uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err);
+pxc_status pxc_bq_session_decode(pxc_bq_session* session, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
+                                 int32_t dtype, uint64_t stride, void* stream, pxc_error* err);
+pxc_status pxc_bq_session_product(pxc_bq_session* session, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
+                                  uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream,
+                                  pxc_error* err);
+pxc_status pxc_bq_session_grouped_product(pxc_bq_session* session, const pxc_bq_rows* d_queries,
+                                          const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
+                                          const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
+                                          int32_t dtype, uint64_t size, void* stream, pxc_error* err);
+/* Reports a failure that is known already, without waiting. */
+pxc_status pxc_bq_session_report(pxc_bq_session* session, pxc_error* err);
+/* Waits for `stream` (NULL: the context's) and reports a failure that the session's
+ * calls left, on whichever stream, or that calls with the context itself left on this one. */
+pxc_status pxc_bq_session_check(pxc_bq_session* session, void* stream, pxc_error* err);
 
 #ifdef __cplusplus
 }

@@ -14,12 +14,13 @@ that probe an inverted list with the list's rows, a tenant's queries with the te
 rows, or the tokens of an expert with the expert's weights.
 
 CUDA tensors in give CUDA tensors out, computed on the current stream without a wait; a
-failure that only the device sees (bad offsets) is raised by a later call or by
-``check()``. Host arrays in give NumPy arrays out. There is no CPU path.
+failure that only the device sees (bad offsets) is raised by a later call of the same quantiser, or by its
+``check()``, and by nobody else's: callers in several threads have a quantiser each. Host arrays in give NumPy arrays out. There is no CPU path.
 """
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 from typing import Any
 
@@ -60,8 +61,8 @@ class _Torch:
         self.uint8, self.int64, self.float32, self.empty = torch.uint8, torch.int64, torch.float32, torch.empty
         self.current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
-        self.encode, self.decode = N.bind("pxc_bq_encode_device"), N.bind("pxc_bq_decode_device")
-        self.product, self.grouped = N.bind("pxc_bq_product_device"), N.bind("pxc_bq_grouped_product_device")
+        self.encode, self.decode = N.bind("pxc_bq_session_encode"), N.bind("pxc_bq_session_decode")
+        self.product, self.grouped = N.bind("pxc_bq_session_product"), N.bind("pxc_bq_session_grouped_product")
 
 
 _torch_parts: _Torch | None = None
@@ -72,6 +73,21 @@ def _torch() -> _Torch:
     if _torch_parts is None:
         _torch_parts = _Torch()
     return _torch_parts
+
+
+class _Session:
+    """The native record of a quantiser's failures (pxc_bq_session)."""
+
+    def __init__(self, context):
+        handle = N.vp()
+        N.call("pxc_bq_session_create", context.handle, C.byref(handle))
+        self.handle = handle.value
+
+    def __del__(self):
+        try:
+            N.load().pxc_bq_session_destroy(self.handle)
+        except Exception:
+            pass
 
 
 @dataclass(slots=True)
@@ -111,6 +127,19 @@ class BlockQuantizer:
         self.ctx = context
         self.blocks = -(-dim // BLOCK)
         self._ld, self._sld = (dim + 15) & ~15, (self.blocks + 3) & ~3
+        self._session = None
+        self._opening = threading.Lock()
+
+    def _open(self) -> _Session:
+        with self._opening:
+            if self._session is None:
+                self._session = _Session(self.ctx)
+        return self._session
+
+    def _host(self, name: str, *args) -> None:
+        """A host form, which reports its own failure; what tensors' calls left is raised first."""
+        N.call("pxc_bq_session_report", (self._session or self._open()).handle)
+        N.call(name, self.ctx.handle, *args)
 
     # -- arguments --
     def _stream(self, tensor) -> int:
@@ -183,12 +212,12 @@ class BlockQuantizer:
             codes = t.empty(n, ld, dtype=t.uint8, device=v.device)
             scales = codes.new_empty(n, sld)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
-            t.encode(self.ctx.handle, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
+            t.encode((self._session or self._open()).handle, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
             return BlockCodes(codes, scales, dim)
         v = np.ascontiguousarray(v)
         codes, scales = np.zeros((n, ld), np.uint8), np.zeros((n, sld), np.uint8)
         rows = N.PxcBqRows(N.ptr(codes), N.ptr(scales), n, ld, sld)
-        N.call("pxc_bq_encode", self.ctx.handle, N.ptr(v), _dtype_code(v.dtype), self.dim, self.dim, C.byref(rows))
+        self._host("pxc_bq_encode", N.ptr(v), _dtype_code(v.dtype), self.dim, self.dim, C.byref(rows))
         return BlockCodes(codes, scales, self.dim)
 
     def decode(self, codes: BlockCodes, dtype=None):
@@ -199,10 +228,11 @@ class BlockQuantizer:
             t = _torch()
             code = _dtype_code(dtype or t.float32)
             out = t.empty(rows.rows, self.dim, dtype=dtype or t.float32, device=codes.codes.device)
-            t.decode(self.ctx.handle, C.byref(rows), self.dim, out.data_ptr(), code, self.dim, self._stream(out))
+            t.decode((self._session or self._open()).handle, C.byref(rows), self.dim, out.data_ptr(), code, self.dim,
+                     self._stream(out))
             return out
         out = np.zeros((len(codes), self.dim), dtype or np.float32)
-        N.call("pxc_bq_decode", self.ctx.handle, C.byref(rows), self.dim, N.ptr(out), _dtype_code(out.dtype), self.dim)
+        self._host("pxc_bq_decode", C.byref(rows), self.dim, N.ptr(out), _dtype_code(out.dtype), self.dim)
         return out
 
     # -- products --
@@ -224,12 +254,13 @@ class BlockQuantizer:
                     raise Configuration("out", 0, "must be (nq, n) on the operands' device, with contiguous rows")
                 code = _dtype_code(out.dtype)
                 stride = out.stride(0) if shape[0] > 1 else stride
-            t.product(self.ctx.handle, C.byref(q), C.byref(b), self.dim, out.data_ptr(), code, stride, self._stream(out))
+            t.product((self._session or self._open()).handle, C.byref(q), C.byref(b), self.dim, out.data_ptr(), code,
+                      stride, self._stream(out))
             return out
         if out is not None:
             raise Configuration("out", 0, "is for tensors")
         out = np.zeros(shape, dtype or np.float32)
-        N.call("pxc_bq_product", self.ctx.handle, C.byref(q), C.byref(b), self.dim, N.ptr(out), _dtype_code(out.dtype),
+        self._host("pxc_bq_product", C.byref(q), C.byref(b), self.dim, N.ptr(out), _dtype_code(out.dtype),
                max(shape[1], 1))
         return out
 
@@ -265,11 +296,11 @@ class BlockQuantizer:
             t = _torch()
             code = _dtype_code(dtype or t.float32)
             out = t.empty(*shape, dtype=dtype or t.float32, device=dev)
-            t.grouped(self.ctx.handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups, self.dim, out.data_ptr(),
-                      code, size, self._stream(out))
+            t.grouped((self._session or self._open()).handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups,
+                      self.dim, out.data_ptr(), code, size, self._stream(out))
             return out
         out = np.zeros(shape, dtype or np.float32)
-        N.call("pxc_bq_grouped_product", self.ctx.handle, C.byref(q), N.ptr(qo), C.byref(b), N.ptr(bo), groups, self.dim,
+        self._host("pxc_bq_grouped_product", C.byref(q), N.ptr(qo), C.byref(b), N.ptr(bo), groups, self.dim,
                N.ptr(out), _dtype_code(out.dtype), size)
         return out
 
@@ -283,5 +314,7 @@ class BlockQuantizer:
         return np.ascontiguousarray(o, np.int64)
 
     def check(self) -> None:
-        """Waits for the current stream and raises a failure that an earlier call left on the device."""
-        N.call("pxc_bq_check", self.ctx.handle, _torch().current_stream(self.ctx.device) or 1)
+        """Waits for the current stream and raises a failure that an earlier call of this quantiser left on the
+        device, or one that calls of the C functions with its context left on this stream."""
+        session = self._session or self._open()
+        N.call("pxc_bq_session_check", session.handle, _torch().current_stream(self.ctx.device) or 1)

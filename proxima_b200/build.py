@@ -34,7 +34,8 @@ CUDA_SOURCES = ["ctx.cu", "flat.cu", "kmeans.cu", "ivfpq.cu", "sq.cu", "filter.c
                 "bq.cu"]
 HEADERS = ["common.cuh", "sm100.cuh", "flat_tc.cuh", "topk.cuh", "tmap.cuh", "kmeans_tc.cuh",
            "seqsum.cuh", "rng.h", "kmeans_api.h", "select.cuh", "refdist.cuh", "sq_tc.cuh", "fp32scan.cuh",
-           "ivfpq.cuh", "hostcopy.cuh", "bq.cuh", "bq_tc.cuh"]
+           "ivfpq.cuh", "hostcopy.cuh", "bq.cuh", "bq_tc.cuh",
+           "bq_reports.cuh"]
 CXX = os.environ.get("CXX", shutil.which("g++") or "g++")
 
 

@@ -1,6 +1,7 @@
 // bq.cu — the block quantiser (pxc_bq_*): encode, decode, the product of two sets of
 // encoded rows, and the product grouped by ragged lists.
 #include <algorithm>
+#include <memory>
 #include <type_traits>
 
 #include "bq.cuh"
@@ -365,8 +366,39 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---- host ----
-static void check_common(const pxc_ctx* ctx, uint32_t dim, int32_t dtype) {
-  PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
+// Who makes a call of the device forms, on which stream, and whose failures it reports.
+struct Caller {
+  pxc_ctx* ctx;
+  cudaStream_t stream;
+  Record record;    // what this call's kernels write
+  Record told[2];   // earlier failures that the call reports
+
+  Caller(pxc_ctx* c, void* s) : ctx(c) {
+    PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
+    stream = s ? static_cast<cudaStream_t>(s) : ctx->stream;
+    Reports& reports = *ctx->bq_reports;
+    told[0] = record = reports.of_stream(stream);
+    told[1] = reports.captured();
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess)
+      cudaGetLastError();  // the launch will say what is wrong
+    else if (status != cudaStreamCaptureStatusNone)
+      record = reports.captured();
+  }
+  Caller(pxc_bq_session* session, void* s) {
+    PXC_CONFIG(session != nullptr, "session", 0, "null session");
+    ctx = session->reports->context();
+    PXC_CONFIG(ctx != nullptr, "ctx", 0, "the session's context has gone");
+    stream = s ? static_cast<cudaStream_t>(s) : ctx->stream;
+    told[0] = record = session->record;
+  }
+  void report() const {
+    for (const Record& r : told)
+      if (r.words) r.take();
+  }
+};
+
+static void check_common(uint32_t dim, int32_t dtype) {
   PXC_CONFIG(dim >= 1 && dim <= MAX_DIM, "dim", dim, "must be between 1 and 1048576");
   PXC_CONFIG(dtype == PXC_DTYPE_F32 || dtype == PXC_DTYPE_F16 || dtype == PXC_DTYPE_BF16, "dtype", dtype,
              "must be f32, f16 or bf16");
@@ -386,19 +418,6 @@ static void check_rows(const pxc_bq_rows* r, uint32_t dim, const char* name, boo
              "the code pitch must be a multiple of 16, at least dim and below 2^32");
   PXC_CONFIG(r->sld >= blocks_of(dim) && (r->sld & 3) == 0 && r->sld < (uint64_t(1) << 32), "sld", r->sld,
              "the scale pitch must be a multiple of 4, at least ceil(dim / 128) and below 2^32");
-}
-
-// Reports a failure that an earlier device call left, once.
-static void take_fault(pxc_ctx* ctx) {
-  bool set[FAULT_WORDS];
-  for (uint32_t i = 0; i < FAULT_WORDS; ++i)
-    set[i] = __atomic_load_n(ctx->bq_faults + i, __ATOMIC_RELAXED) != 0 &&
-             __atomic_exchange_n(ctx->bq_faults + i, 0u, __ATOMIC_RELAXED) != 0;
-  if (set[FAULT_TIMEOUT])
-    throw make_failure(PXC_TIMEOUT, 0, 0, nullptr, "a device-side wait of a block product ran out");
-  if (set[FAULT_OFFSETS])
-    throw make_failure(PXC_CONFIGURATION, 0, 0, "offsets",
-                       "a grouped product's offsets fell, left the rows, or did not fit the output");
 }
 
 static void count_launch(pxc_ctx* ctx) { __atomic_fetch_add(&ctx->launches, 1ull, __ATOMIC_RELAXED); }
@@ -516,13 +535,13 @@ static Shape dense_shape(uint64_t nq, uint64_t rows, uint32_t kblocks, uint64_t 
 }
 
 static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, uint32_t dim, const Groups& g, void* out,
-                    int32_t dtype, cudaStream_t s) {
+                    int32_t dtype, cudaStream_t s, const Record& record) {
   using namespace bq_tc;
   Params p{};
   p.groups = g;
   p.groups.nq = q.rows;
   p.groups.nb = b.rows;
-  p.groups.faults = ctx->bq_faults;
+  p.groups.record = record;
   p.q_scales = q.scales;
   p.b_scales = b.scales;
   p.q_sld = q.sld;
@@ -666,10 +685,61 @@ static void check_host_offsets(const int64_t* o, uint32_t groups, uint64_t rows)
                "offsets must rise and stay within the rows");
 }
 
-static void finish(pxc_ctx* ctx, cudaStream_t s) {
-  PXC_CUDA(cudaStreamSynchronize(s));
-  take_fault(ctx);
+// ---- the device forms, of a context's or a session's caller ----
+static void encode_device(const Caller& c, const void* vectors, int32_t dtype, uint64_t stride, uint32_t dim,
+                          const pxc_bq_rows* out) {
+  check_common(dim, dtype);
+  c.report();
+  check_rows(out, dim, "out", true);
+  if (out->rows == 0) return;
+  check_vectors(vectors, dtype, stride, dim, "vectors");
+  DeviceGuard g(c.ctx->device);
+  encode(c.ctx, vectors, dtype, stride, dim, *out, c.stream);
 }
+
+static void decode_device(const Caller& c, const pxc_bq_rows* rows, uint32_t dim, void* out, int32_t dtype,
+                          uint64_t stride) {
+  check_common(dim, dtype);
+  c.report();
+  check_rows(rows, dim, "rows", true);
+  if (rows->rows == 0) return;
+  check_vectors(out, dtype, stride, dim, "out");
+  DeviceGuard g(c.ctx->device);
+  decode(c.ctx, *rows, dim, out, dtype, stride, c.stream);
+}
+
+static void product_device(const Caller& c, const pxc_bq_rows* queries, const pxc_bq_rows* base, uint32_t dim, void* out,
+                           int32_t dtype, uint64_t stride) {
+  check_common(dim, dtype);
+  c.report();
+  check_product(queries, base, dim, out, dtype, stride, true);
+  if (queries->rows == 0 || base->rows == 0) return;
+  DeviceGuard g(c.ctx->device);
+  Groups groups{};
+  groups.groups = 1;
+  groups.n_each = base->rows;
+  groups.stride = stride;
+  product(c.ctx, *queries, *base, dim, groups, out, dtype, c.stream, c.record);
+}
+
+static void grouped_device(const Caller& c, const pxc_bq_rows* queries, const int64_t* query_offsets,
+                           const pxc_bq_rows* base, const int64_t* base_offsets, uint32_t groups, uint32_t dim, void* out,
+                           int32_t dtype, uint64_t size) {
+  check_common(dim, dtype);
+  c.report();
+  const uint64_t each = check_grouped(queries, query_offsets, base, base_offsets, groups, dim, out, dtype, size, true);
+  if (queries->rows == 0 || base->rows == 0 || size == 0) return;
+  DeviceGuard g(c.ctx->device);
+  Groups gr{};
+  gr.q_offsets = query_offsets;
+  gr.b_offsets = base_offsets;
+  gr.groups = groups;
+  gr.n_each = gr.stride = each;
+  gr.size = size;
+  product(c.ctx, *queries, *base, dim, gr, out, dtype, c.stream, c.record);
+}
+
+static void check_context(const pxc_ctx* ctx) { PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context"); }
 
 }  // namespace bq
 }  // namespace pxc
@@ -681,21 +751,15 @@ extern "C" {
 pxc_status pxc_bq_encode_device(pxc_ctx* ctx, const void* d_vectors, int32_t dtype, uint64_t stride, uint32_t dim,
                                 const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
-    bq::check_rows(d_out, dim, "out", true);
-    if (d_out->rows == 0) return;
-    bq::check_vectors(d_vectors, dtype, stride, dim, "vectors");
-    DeviceGuard g(ctx->device);
-    bq::encode(ctx, d_vectors, dtype, stride, dim, *d_out, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    bq::encode_device(bq::Caller(ctx, stream), d_vectors, dtype, stride, dim, d_out);
   });
 }
 
 pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint64_t stride, uint32_t dim,
                          const pxc_bq_rows* out, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
+    bq::check_context(ctx);
+    bq::check_common(dim, dtype);
     bq::check_rows(out, dim, "out", false);
     if (out->rows == 0) return;
     bq::check_vectors(vectors, dtype, stride, dim, "vectors");
@@ -718,21 +782,15 @@ pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint6
 pxc_status pxc_bq_decode_device(pxc_ctx* ctx, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out, int32_t dtype,
                                 uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
-    bq::check_rows(d_rows, dim, "rows", true);
-    if (d_rows->rows == 0) return;
-    bq::check_vectors(d_out, dtype, stride, dim, "out");
-    DeviceGuard g(ctx->device);
-    bq::decode(ctx, *d_rows, dim, d_out, dtype, stride, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    bq::decode_device(bq::Caller(ctx, stream), d_rows, dim, d_out, dtype, stride);
   });
 }
 
 pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, void* out, int32_t dtype, uint64_t stride,
                          pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
+    bq::check_context(ctx);
+    bq::check_common(dim, dtype);
     bq::check_rows(rows, dim, "rows", false);
     if (rows->rows == 0) return;
     bq::check_vectors(out, dtype, stride, dim, "out");
@@ -753,29 +811,20 @@ pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, vo
 pxc_status pxc_bq_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base, uint32_t dim,
                                  void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
-    bq::check_product(d_queries, d_base, dim, d_out, dtype, stride, true);
-    if (d_queries->rows == 0 || d_base->rows == 0) return;
-    DeviceGuard g(ctx->device);
-    bq::Groups groups{};
-    groups.groups = 1;
-    groups.n_each = d_base->rows;
-    groups.stride = stride;
-    bq::product(ctx, *d_queries, *d_base, dim, groups, d_out, dtype,
-                stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    bq::product_device(bq::Caller(ctx, stream), d_queries, d_base, dim, d_out, dtype, stride);
   });
 }
 
 pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq_rows* base, uint32_t dim, void* out,
                           int32_t dtype, uint64_t stride, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
+    bq::check_context(ctx);
+    bq::check_common(dim, dtype);
     bq::check_product(queries, base, dim, out, dtype, stride, false);
     if (queries->rows == 0 || base->rows == 0) return;
     std::lock_guard<std::mutex> lock(ctx->mu);
     DeviceGuard g(ctx->device);
+    const bq::Leased mine(*ctx->bq_reports);
     cudaStream_t s = ctx->stream;
     const size_t es = bq::size_of(dtype);
     bq::Staged q, b;
@@ -786,9 +835,10 @@ pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq
     bq::Groups groups{};
     groups.groups = 1;
     groups.n_each = groups.stride = base->rows;
-    bq::product(ctx, q.d, b.d, dim, groups, o.p, dtype, s);
+    bq::product(ctx, q.d, b.d, dim, groups, o.p, dtype, s, mine.record);
     bq::copy_rows(out, stride * es, o.p, base->rows * es, base->rows * es, queries->rows, cudaMemcpyDeviceToHost, s);
-    bq::finish(ctx, s);
+    PXC_CUDA(cudaStreamSynchronize(s));
+    mine.record.take();
   });
 }
 
@@ -797,20 +847,8 @@ pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_quer
                                          uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
                                          pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
-    const uint64_t each =
-        bq::check_grouped(d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim, d_out, dtype, size, true);
-    if (d_queries->rows == 0 || d_base->rows == 0 || size == 0) return;
-    DeviceGuard g(ctx->device);
-    bq::Groups gr{};
-    gr.q_offsets = d_query_offsets;
-    gr.b_offsets = d_base_offsets;
-    gr.groups = groups;
-    gr.n_each = gr.stride = each;
-    gr.size = size;
-    bq::product(ctx, *d_queries, *d_base, dim, gr, d_out, dtype,
-                stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    bq::grouped_device(bq::Caller(ctx, stream), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim, d_out,
+                       dtype, size);
   });
 }
 
@@ -818,8 +856,8 @@ pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, cons
                                   const pxc_bq_rows* base, const int64_t* base_offsets, uint32_t groups, uint32_t dim,
                                   void* out, int32_t dtype, uint64_t size, pxc_error* err) {
   return guarded(err, [&] {
-    bq::check_common(ctx, dim, dtype);
-    bq::take_fault(ctx);
+    bq::check_context(ctx);
+    bq::check_common(dim, dtype);
     const uint64_t each = bq::check_grouped(queries, query_offsets, base, base_offsets, groups, dim, out, dtype, size, false);
     bq::check_host_offsets(query_offsets, groups, queries->rows);
     uint64_t need = queries->rows * each;
@@ -835,6 +873,7 @@ pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, cons
     if (need == 0) return;
     std::lock_guard<std::mutex> lock(ctx->mu);
     DeviceGuard g(ctx->device);
+    const bq::Leased mine(*ctx->bq_reports);
     cudaStream_t s = ctx->stream;
     const size_t es = bq::size_of(dtype);
     bq::Staged q, b;
@@ -856,19 +895,84 @@ pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, cons
     gr.groups = groups;
     gr.n_each = gr.stride = each;
     gr.size = need;
-    bq::product(ctx, q.d, b.d, dim, gr, o.p, dtype, s);
+    bq::product(ctx, q.d, b.d, dim, gr, o.p, dtype, s, mine.record);
     if (count)
       PXC_CUDA(cudaMemcpyAsync(static_cast<uint8_t*>(out) + first * es, o.p + first * es, count * es,
                                cudaMemcpyDeviceToHost, s));
-    bq::finish(ctx, s);
+    PXC_CUDA(cudaStreamSynchronize(s));
+    mine.record.take();
   });
 }
 
 pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
+    const bq::Caller c(ctx, stream);
     DeviceGuard g(ctx->device);
-    bq::finish(ctx, stream ? static_cast<cudaStream_t>(stream) : ctx->stream);
+    PXC_CUDA(cudaStreamSynchronize(c.stream));
+    c.report();
+  });
+}
+
+pxc_status pxc_bq_session_create(pxc_ctx* ctx, pxc_bq_session** out, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::check_context(ctx);
+    PXC_CONFIG(out != nullptr, "out", 0, "null output");
+    auto h = std::make_unique<pxc_bq_session>();
+    h->reports = ctx->bq_reports;
+    h->record = h->reports->lease();
+    *out = h.release();
+  });
+}
+
+void pxc_bq_session_destroy(pxc_bq_session* session) {
+  if (!session) return;
+  session->reports->give_back(session->record);
+  delete session;
+}
+
+pxc_status pxc_bq_session_encode(pxc_bq_session* session, const void* d_vectors, int32_t dtype, uint64_t stride,
+                                 uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::encode_device(bq::Caller(session, stream), d_vectors, dtype, stride, dim, d_out);
+  });
+}
+
+pxc_status pxc_bq_session_decode(pxc_bq_session* session, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
+                                 int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::decode_device(bq::Caller(session, stream), d_rows, dim, d_out, dtype, stride);
+  });
+}
+
+pxc_status pxc_bq_session_product(pxc_bq_session* session, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
+                                  uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream,
+                                  pxc_error* err) {
+  return guarded(err, [&] {
+    bq::product_device(bq::Caller(session, stream), d_queries, d_base, dim, d_out, dtype, stride);
+  });
+}
+
+pxc_status pxc_bq_session_grouped_product(pxc_bq_session* session, const pxc_bq_rows* d_queries,
+                                          const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
+                                          const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
+                                          int32_t dtype, uint64_t size, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    bq::grouped_device(bq::Caller(session, stream), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim,
+                       d_out, dtype, size);
+  });
+}
+
+pxc_status pxc_bq_session_report(pxc_bq_session* session, pxc_error* err) {
+  return guarded(err, [&] { bq::Caller(session, nullptr).report(); });
+}
+
+pxc_status pxc_bq_session_check(pxc_bq_session* session, void* stream, pxc_error* err) {
+  return guarded(err, [&] {
+    const bq::Caller c(session, stream);
+    DeviceGuard g(c.ctx->device);
+    PXC_CUDA(cudaStreamSynchronize(c.stream));
+    c.report();
+    c.ctx->bq_reports->of_stream(c.stream).take();
   });
 }
 

@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "bq_reports.cuh"
 #include "common.cuh"
 
 namespace pxc {
@@ -19,11 +20,9 @@ namespace bq {
 
 constexpr uint32_t BLOCK = 128;  // components per scale
 
-// Failures that only the device sees: a word each in pinned host memory, set by the kernel and
-// taken by the next call.
-enum Fault : uint32_t { FAULT_OFFSETS = 0, FAULT_TIMEOUT = 1, FAULT_WORDS = 2 };
-__device__ __forceinline__ void leave_fault(uint32_t* faults, Fault which) {
-  *reinterpret_cast<volatile uint32_t*>(faults + which) = 1;
+// A failure that only the device sees, into the caller's record.
+__device__ __forceinline__ void leave_fault(const Record& r, Fault which) {
+  *reinterpret_cast<volatile uint32_t*>(r.words + which) = r.id;
   __threadfence_system();
 }
 
@@ -88,7 +87,7 @@ struct Groups {
   uint64_t n_each;      // even (and dense): base rows per group, and the output's row pitch is `stride`
   uint64_t stride;
   uint64_t size;        // room in the output, in values (ragged)
-  uint32_t* faults;
+  Record record;        // for failures
 };
 
 // One output tile: `queries` x `rows` values from (q0, b0), the first at out[at].
@@ -218,7 +217,7 @@ struct Walk {
       tile_sum += tiles[j];
     }
     tiles_upto = scan(tile_sum);
-    if (bad) leave_fault(g.faults, FAULT_OFFSETS);
+    if (bad) leave_fault(g.record, FAULT_OFFSETS);
     if (g.groups - chunk > CHUNK) fetch(static_cast<uint64_t>(chunk) + CHUNK);
   }
 

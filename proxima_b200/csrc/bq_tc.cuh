@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   tc_fence_after();
   if (warp == 1) tmem_free<G>(tmem);
-  if (threadIdx.x == 0 && c.failed) leave_fault(p.groups.faults, FAULT_TIMEOUT);
+  if (threadIdx.x == 0 && c.failed) leave_fault(p.groups.record, FAULT_TIMEOUT);
 }
 
 }  // namespace bq_tc

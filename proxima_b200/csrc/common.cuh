@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 
 #include "proxima_cuda.h"
@@ -124,6 +125,12 @@ enum DeviceError : uint32_t {
 
 }  // namespace pxc
 
+namespace pxc {
+namespace bq {
+class Reports;
+}
+}  // namespace pxc
+
 // ---------------------------------------------------------------------------
 // Context: one device, one default stream, a small device error/status area.
 // ---------------------------------------------------------------------------
@@ -133,7 +140,7 @@ struct pxc_ctx {
   uint32_t wait_ms = 2000;
   uint32_t* d_status = nullptr;  // [0] device error word, [1] aux
   uint32_t* h_status = nullptr;  // pinned mirror
-  uint32_t* bq_faults = nullptr;  // pinned: failures that a block product's kernel left (bq.cuh)
+  std::shared_ptr<pxc::bq::Reports> bq_reports;  // failures of block products (bq_reports.cuh)
   uint32_t bq_ready = 0;          // block product kernels (a bit each) set up on the device
   int sm_count = 0;
   bool profiling = false;

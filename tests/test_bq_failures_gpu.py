@@ -56,3 +56,234 @@ def test_a_failed_product_ends_soon_and_leaves_nothing_behind(ctx, nq, n):
         ctx.set_wait_limit(2000)
         assert torch.equal(bq.product(c[:nq], c[:n]), want)
         bq.check()
+
+
+# ---- who is told ----
+BAD = [0, 30, 20]  # query offsets that fall
+
+
+def some_codes(bq, rows, seed):
+    g = torch.Generator().manual_seed(seed)
+    return bq.encode(torch.randint(-3, 4, (rows, bq.dim), generator=g).float().cuda())
+
+
+def bad_call(bq, q, b):
+    bq.grouped_product(q, torch.tensor(BAD, device="cuda"), b)
+
+
+def test_a_quantiser_hears_of_its_own_calls_alone(ctx):
+    a, b = BlockQuantizer(48, context=ctx), BlockQuantizer(48, context=ctx)
+    q, base = some_codes(a, 20, 1), some_codes(a, 40, 2)
+    want = b.product(q, base)
+    bad_call(a, q, base)
+    torch.cuda.synchronize()
+    # every kind of call of another quantiser on the same context and stream
+    x = b.decode(q)
+    b.encode(x)
+    assert torch.equal(b.product(q, base), want)
+    b.grouped_product(q, torch.tensor([0, 5, 20], device="cuda"), base)
+    host = b.encode(x.cpu().numpy())
+    assert np.array_equal(b.product(host, host), b.product(q, q).cpu().numpy())
+    b.check()
+    with pytest.raises(Configuration) as e:
+        a.check()
+    assert e.value.parameter == "offsets"
+    a.check()  # once
+    # and the one that failed hears of it from each kind of call
+    for call in (lambda: a.encode(x), lambda: a.decode(q), lambda: a.product(q, base),
+                 lambda: a.grouped_product(q, torch.tensor([0, 20], device="cuda"), base),
+                 lambda: a.encode(x.cpu().numpy()), lambda: a.product(host, host)):
+        bad_call(a, q, base)
+        torch.cuda.synchronize()
+        with pytest.raises(Configuration):
+            call()
+        call()
+
+
+def test_two_threads_of_which_one_fails(ctx):
+    import threading
+
+    rounds = 200
+    setup = BlockQuantizer(48, context=ctx)
+    q, base = some_codes(setup, 20, 1), some_codes(setup, 40, 2)
+    want = setup.product(q, base)
+    torch.cuda.synchronize()
+    problems, told = [], []
+
+    def bad():
+        try:
+            bq = BlockQuantizer(48, context=ctx)
+            for _ in range(rounds):
+                bad_call(bq, q, base)
+                try:
+                    bq.check()
+                except Configuration:
+                    told.append(1)
+        except BaseException as e:
+            problems.append(e)
+
+    def good():
+        try:
+            bq = BlockQuantizer(48, context=ctx)
+            results = []
+            for _ in range(rounds):
+                results.append(bq.product(q, base))
+                bq.check()
+            assert len(results) == rounds and all(torch.equal(r, want) for r in results)
+        except BaseException as e:
+            problems.append(e)
+
+    threads = [threading.Thread(target=f) for f in (bad, good, good)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not problems and len(told) == rounds
+
+
+def test_calls_on_the_context_are_told_by_stream(ctx):
+    bq = BlockQuantizer(48, context=ctx)
+    q, base = some_codes(bq, 20, 1), some_codes(bq, 40, 2)
+    rq, rb = bq._rows(q, True, "q"), bq._rows(base, True, "b")
+    out = torch.zeros(2000, device="cuda")
+    off = torch.tensor(BAD, device="cuda")
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def bad(stream):
+        N.call("pxc_bq_grouped_product_device", ctx.handle, C.byref(rq), off.data_ptr(), C.byref(rb), None, 2, 48,
+               out.data_ptr(), 0, 2000, stream.cuda_stream)
+
+    bad(one)
+    torch.cuda.synchronize()
+    N.call("pxc_bq_product_device", ctx.handle, C.byref(rq), C.byref(rb), 48, out.data_ptr(), 0, 40, two.cuda_stream)
+    N.call("pxc_bq_check", ctx.handle, two.cuda_stream)
+    N.call("pxc_bq_check", ctx.handle, None)
+    bq.check()
+    host = BlockCodes(q.codes.cpu().numpy(), q.scales.cpu().numpy(), 48)
+    bq.product(host, host)
+    with pytest.raises(Configuration):
+        N.call("pxc_bq_check", ctx.handle, one.cuda_stream)
+    N.call("pxc_bq_check", ctx.handle, one.cuda_stream)
+    bad(one)
+    torch.cuda.synchronize()
+    with pytest.raises(Configuration):  # the next call there
+        N.call("pxc_bq_product_device", ctx.handle, C.byref(rq), C.byref(rb), 48, out.data_ptr(), 0, 40, one.cuda_stream)
+    # of a graph, which may run on any stream: any call on the context itself
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=one):
+        bad(one)
+    with torch.cuda.stream(two):
+        graph.replay()
+    torch.cuda.synchronize()
+    BlockQuantizer(48, context=ctx).product(q, base)
+    with pytest.raises(Configuration):
+        N.call("pxc_bq_check", ctx.handle, None)
+
+
+def test_a_host_call_that_fails_says_so_whatever_others_do(ctx):
+    """Products of host rows whose wait runs out, beside a thread of calls that succeed on the same context."""
+    import threading
+
+    bq = BlockQuantizer(LONG, context=ctx)
+    c = BlockCodes(np.full((224, LONG), 0x38, np.uint8), np.full((224, LONG // 128), 127, np.uint8), LONG)
+    small = BlockQuantizer(48, context=ctx)
+    q = some_codes(small, 20, 1)
+    torch.cuda.synchronize()
+    stop, problems, calls = threading.Event(), [], []
+
+    def others():
+        try:
+            while not stop.is_set():
+                small.encode(small.decode(q))
+                small.check()
+                calls.append(1)
+        except BaseException as e:
+            problems.append(e)
+
+    ctx.set_wait_limit(1)
+    t = threading.Thread(target=others)
+    t.start()
+    try:
+        for _ in range(8):
+            with pytest.raises(DeviceTimeout):
+                bq.product(c, c)
+    finally:
+        stop.set()
+        t.join()
+        ctx.set_wait_limit(2000)
+    assert not problems and calls
+    bq.check()
+    assert (bq.product(c[:3], c) == LONG).all()
+
+
+def test_two_kinds_of_failure_are_both_told(ctx):
+    bq = BlockQuantizer(LONG, context=ctx)
+    c = ones(224, LONG)
+    small = BlockCodes(c.codes[:40], c.scales[:40], LONG)
+    bq.product(small, small)
+    graph = torch.cuda.CUDAGraph()  # as no call may come between the two
+    off, whole = torch.tensor([0, 30, 20], device="cuda"), torch.tensor([0, 224], device="cuda")
+    ctx.set_wait_limit(1)
+    with torch.cuda.graph(graph):
+        bq.grouped_product(small, off, small)
+        bq.grouped_product(c, whole, c)
+    ctx.set_wait_limit(2000)
+    graph.replay()
+    with pytest.raises(DeviceTimeout):
+        bq.check()
+    with pytest.raises(Configuration):
+        bq.check()
+    bq.check()
+
+
+def test_graphs_report_to_the_quantiser_that_was_captured(ctx):
+    a, b = BlockQuantizer(48, context=ctx), BlockQuantizer(48, context=ctx)
+    q, base = some_codes(a, 20, 1), some_codes(a, 40, 2)
+    off = torch.tensor([0, 10, 20], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.grouped_product(q, off, base)
+    graph.replay()
+    a.check()
+    off.copy_(torch.tensor(BAD))
+    with torch.cuda.stream(torch.cuda.Stream()):
+        graph.replay()
+        torch.cuda.synchronize()
+    b.check()
+    with pytest.raises(Configuration):
+        a.product(q, base)
+
+
+def test_quantisers_that_come_and_go(ctx):
+    """A quantiser may go before its work has run; nobody else is told of it, and there are many."""
+    first = BlockQuantizer(48, context=ctx)
+    q, base = some_codes(first, 20, 1), some_codes(first, 40, 2)
+    want = first.product(q, base)
+    kept = []
+    for i in range(3000):
+        bad_call(BlockQuantizer(48, context=ctx), q, base)
+        later = BlockQuantizer(48, context=ctx)
+        if i % 100 == 0:
+            assert torch.equal(later.product(q, base), want)
+            kept.append(later)
+    for k in kept:
+        k.check()
+    first.check()
+    bad_call(kept[3], q, base)
+    for k in kept[:3] + kept[4:]:
+        k.check()
+    with pytest.raises(Configuration):
+        kept[3].check()
+
+
+def test_a_closed_context_is_refused():
+    ctx = Context(0)
+    bq = BlockQuantizer(48, context=ctx)
+    q = some_codes(bq, 20, 1)
+    torch.cuda.synchronize()
+    ctx.close()
+    for call in (lambda: bq.decode(q), lambda: bq.product(q, q), bq.check,
+                 lambda: BlockQuantizer(48, context=ctx).decode(q)):
+        with pytest.raises(Configuration):
+            call()
