@@ -107,8 +107,9 @@ struct Tile {
 // L2 while the queries pass.
 //
 // Every group is checked before it counts: its offsets rise and lie within the rows, and its
-// matrix ends within the output. One that fails counts as empty and leaves a fault, so
-// that no offsets lead to an access out of range, and the number of tiles is at most that of output values.
+// matrix ends within the output. One that fails leaves a fault, and it and all groups behind it count as
+// empty. So no offsets lead to an access out of range, the groups that count are disjoint in rows and outputs, and
+// the number of tiles is at most that of output values.
 struct Walk {
   static constexpr uint32_t PANEL = 64, PER = 4, CHUNK = 32 * PER;
   const Groups& g;
@@ -117,6 +118,7 @@ struct Walk {
   uint32_t chunk = 0;
   uint64_t tiles_before = 0, values_before = 0;  // of earlier chunks
   uint64_t tiles_upto = 0, values_upto = 0;      // of this one, up to and with this lane's groups
+  bool stopped = false;                          // at a group whose offsets are no good
   // this lane's groups: first rows, sizes, tiles and output values
   uint32_t q0[PER], b0[PER], m[PER], n[PER];
   uint64_t tiles[PER], values[PER];
@@ -183,7 +185,7 @@ struct Walk {
   }
 
   __device__ __forceinline__ void load() {
-    bool bad = false;
+    bool bad = false;  // a group of this lane, or one before
     uint64_t value_sum = 0, tile_sum = 0;
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
@@ -195,8 +197,16 @@ struct Walk {
       n[j] = g.b_offsets ? static_cast<uint32_t>(b_next[j + 1]) - b0[j] : there ? static_cast<uint32_t>(g.n_each) : 0u;
       const bool good =
           within(q_next[j], q_next[j + 1], g.nq) && (!g.b_offsets || within(b_next[j], b_next[j + 1], g.nb));
-      if (!good) m[j] = n[j] = 0;
       bad = bad || (there && !good);
+      if (bad || !good) m[j] = n[j] = 0;
+    }
+    const uint32_t bad_lanes = __ballot_sync(0xFFFFFFFFu, bad);
+    if (bad_lanes != 0) leave_fault(g.record, FAULT_OFFSETS);
+    const bool behind = stopped || (bad_lanes & ((1u << lane) - 1)) != 0;
+    stopped = stopped || bad_lanes != 0;
+#pragma unroll
+    for (uint32_t j = 0; j < PER; ++j) {
+      if (behind) m[j] = n[j] = 0;
       // m, n < 2^31 and size <= 2^48: with each term held to size + 1 no sum overflows, and one that is past the
       // room stays past it for all groups behind
       values[j] = g.b_offsets ? min(static_cast<uint64_t>(m[j]) * n[j], g.size + 1) : 0;
@@ -205,11 +215,13 @@ struct Walk {
     if (g.b_offsets) {
       values_upto = scan(value_sum);
       uint64_t upto = values_before + values_upto - value_sum;
+      bool past = false;
 #pragma unroll
       for (uint32_t j = 0; j < PER; ++j) {
         upto += values[j];
-        if (values[j] != 0 && upto > g.size) bad = true, m[j] = 0;
+        if (values[j] != 0 && upto > g.size) past = true, m[j] = 0;
       }
+      if (past) leave_fault(g.record, FAULT_OFFSETS);
     }
 #pragma unroll
     for (uint32_t j = 0; j < PER; ++j) {
@@ -217,7 +229,6 @@ struct Walk {
       tile_sum += tiles[j];
     }
     tiles_upto = scan(tile_sum);
-    if (bad) leave_fault(g.record, FAULT_OFFSETS);
     if (g.groups - chunk > CHUNK) fetch(static_cast<uint64_t>(chunk) + CHUNK);
   }
 
@@ -265,7 +276,7 @@ struct Walk {
       if (t < tiles_before + total) break;
       tiles_before += total;
       values_before = min(values_before + __shfl_sync(0xFFFFFFFFu, values_upto, 31), uint64_t(1) << 60);
-      if (g.groups - chunk <= CHUNK) {
+      if (stopped || g.groups - chunk <= CHUNK) {
         chunk = g.groups;  // nothing behind: later calls find nothing either
         tiles_upto = values_upto = 0;
         return false;

@@ -287,3 +287,47 @@ def test_a_closed_context_is_refused():
                  lambda: BlockQuantizer(48, context=ctx).decode(q)):
         with pytest.raises(Configuration):
             call()
+
+
+# ---- offsets ----
+def test_groups_behind_a_bad_one_do_no_work(ctx):
+    """Offsets that go up and down: every other group would pair all queries with its rows. Only those before the
+    first fall count, so the work is that of one group and not that of half a million (45 million tiles)."""
+    groups, nq, dim = 1 << 20, 20_000, 16
+    bq = BlockQuantizer(dim, context=ctx)
+    q, base = some_codes(bq, nq, 1), some_codes(bq, groups, 2)
+    off = torch.zeros(groups + 1, dtype=torch.int64, device="cuda")
+    bq.grouped_product(q, off, base)
+    off[1::2] = nq
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    got = bq.grouped_product(q, off, base)
+    end.record()
+    with pytest.raises(Configuration):
+        bq.check()
+    assert start.elapsed_time(end) < 30.0
+    assert got.shape == (nq, 1)
+
+
+@pytest.mark.parametrize("bad", [0, 1, 3, 4, 127, 128, 131, 300, 511])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_groups_before_a_bad_one_are_whole_and_those_behind_are_not_written(ctx, bad, ragged):
+    """512 groups of 3 queries and 2 rows, of which one has offsets that fall."""
+    groups, dim = 512, 32
+    bq = BlockQuantizer(dim, context=ctx)
+    q, base = some_codes(bq, 3 * groups, 3), some_codes(bq, 2 * groups, 4)
+    r = [bq._rows(x, True, "x") for x in (q, base)]
+    qo, bo = 3 * torch.arange(groups + 1), 2 * torch.arange(groups + 1)
+    good = bq.grouped_product(q, qo.cuda(), base).reshape(-1)
+    qo[bad + 1:] += 5
+    qo[bad] += 9  # past its end
+    out = torch.full((6 * groups,), -9.0, device="cuda")
+    dqo, dbo = qo.cuda(), bo.cuda()
+    N.call("pxc_bq_grouped_product_device", ctx.handle, C.byref(r[0]), dqo.data_ptr(), C.byref(r[1]),
+           dbo.data_ptr() if ragged else None, groups, dim, out.data_ptr(), 0, 6 * groups, 1)
+    with pytest.raises(Configuration):
+        bq.check()
+    before = max(bad - 1, 0)  # the group before ends 9 queries later
+    assert torch.equal(out[:6 * before], good[:6 * before])
+    written = 6 * before + (2 * 12 if bad else 0)
+    assert (out[written:] == -9).all()
