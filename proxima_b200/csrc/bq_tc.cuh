@@ -281,12 +281,15 @@ __device__ __forceinline__ bool wait_one(Control& c, uint64_t* bar, uint32_t par
     }
   }
 }
-// The same for a whole warp.
+// The same for a whole warp. A shuffle orders no memory: what the barrier's signal makes visible to the waiting
+// lane is so for the others behind the warp's barrier.
 template <bool PAIR>
 __device__ __forceinline__ bool wait_warp(Control& c, uint64_t* bar, uint32_t parity, uint64_t limit) {
   bool ok = true;
   if ((threadIdx.x & 31) == 0) ok = wait_one<PAIR>(c, bar, parity, limit);
-  return __shfl_sync(0xFFFFFFFFu, ok, 0);
+  ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+  __syncwarp();
+  return ok;
 }
 // Before the CTA ends, regardless of failures: for what is in flight, at the latest DRAIN_CYCLES after `start`.
 __device__ __forceinline__ void wait_drained(uint64_t* bar, uint32_t parity, uint64_t start) {
