@@ -365,6 +365,20 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// A grouped product of no queries, no rows or no room: its offsets are looked over all the same.
+__global__ void __launch_bounds__(256) check_empty_kernel(Groups g) {
+  bool bad = false;
+  for (uint64_t i = blockIdx.x * blockDim.x + threadIdx.x; i < g.groups; i += gridDim.x * blockDim.x) {
+    const int64_t q0 = g.q_offsets[i], q1 = g.q_offsets[i + 1];
+    bad = bad || !Walk::within(q0, q1, g.nq);
+    if (g.b_offsets) {
+      const int64_t b0 = g.b_offsets[i], b1 = g.b_offsets[i + 1];
+      bad = bad || !Walk::within(b0, b1, g.nb) || (q1 != q0 && b1 != b0);  // a matrix, and no room
+    }
+  }
+  if (bad) leave_fault(g.record, FAULT_OFFSETS);
+}
+
 // ---- host ----
 // Who makes a call of the device forms, on which stream, and whose failures it reports.
 struct Caller {
@@ -728,14 +742,23 @@ static void grouped_device(const Caller& c, const pxc_bq_rows* queries, const in
   check_common(dim, dtype);
   c.report();
   const uint64_t each = check_grouped(queries, query_offsets, base, base_offsets, groups, dim, out, dtype, size, true);
-  if (queries->rows == 0 || base->rows == 0 || size == 0) return;
   DeviceGuard g(c.ctx->device);
   Groups gr{};
+  gr.nq = queries->rows;
+  gr.nb = base->rows;
+  gr.record = c.record;
   gr.q_offsets = query_offsets;
   gr.b_offsets = base_offsets;
   gr.groups = groups;
   gr.n_each = gr.stride = each;
   gr.size = size;
+  if (queries->rows == 0 || base->rows == 0 || size == 0) {
+    const unsigned grid = std::min<unsigned>((groups + 255) / 256, static_cast<unsigned>(c.ctx->sm_count) * 8);
+    check_empty_kernel<<<grid, 256, 0, c.stream>>>(gr);
+    PXC_CUDA(cudaGetLastError());
+    count_launch(c.ctx);
+    return;
+  }
   product(c.ctx, *queries, *base, dim, gr, out, dtype, c.stream, c.record);
 }
 

@@ -331,3 +331,42 @@ def test_groups_before_a_bad_one_are_whole_and_those_behind_are_not_written(ctx,
     assert torch.equal(out[:6 * before], good[:6 * before])
     written = 6 * before + (2 * 12 if bad else 0)
     assert (out[written:] == -9).all()
+
+
+@pytest.mark.parametrize("nq,n,qo,bo,size", [
+    (0, 6, [0, 2], None, 0),  # no queries: past them
+    (0, 6, [0, 0, 0], [0, 7, 6], 0),
+    (5, 0, [0, 6], None, 0),  # no rows
+    (5, 0, [3, 2, 5], [0, 0, 0], 0),
+    (5, 0, [0, 5], [0, 1], 9),
+    (5, 6, [0, 5], [0, 6], 0),  # no room
+    (5, 6, [0, 0, 5], [0, 4, 6], 0),
+    (5, 6, [0] * 700 + [5], [0] * 700 + [6], 0),
+])
+def test_bad_offsets_of_an_empty_product_are_told_too(ctx, nq, n, qo, bo, size):
+    bq = BlockQuantizer(48, context=ctx)
+    q, b = bq.encode(torch.ones((nq, 48), device="cuda")), bq.encode(torch.ones((n, 48), device="cuda"))
+    r = [bq._rows(x, True, "x") for x in (q, b)]
+    off = [o and torch.tensor(o, device="cuda") for o in (qo, bo)]
+    out = torch.full((64,), -9.0, device="cuda")
+    N.call("pxc_bq_grouped_product_device", ctx.handle, C.byref(r[0]), off[0].data_ptr(), C.byref(r[1]), N.ptr(off[1]),
+           len(qo) - 1, 48, out.data_ptr(), 0, size, 1)
+    with pytest.raises(Configuration) as e:
+        bq.check()
+    assert e.value.parameter == "offsets" and (out == -9).all()
+    if bo is not None:
+        bq.grouped_product(q, off[0], b, off[1], out_size=size)
+        with pytest.raises(Configuration):
+            bq.check()
+
+
+@pytest.mark.parametrize("nq,n,qo,bo,size", [
+    (0, 6, [0, 0, 0], None, 0), (0, 6, [0, 0], [2, 5], 0), (5, 0, [1, 4], None, 0), (5, 0, [0, 5], [0, 0], 7),
+    (5, 6, [0, 0, 5], [0, 4, 4], 0),
+])
+def test_good_offsets_of_an_empty_product_are_no_failure(ctx, nq, n, qo, bo, size):
+    bq = BlockQuantizer(48, context=ctx)
+    q, b = bq.encode(torch.ones((nq, 48), device="cuda")), bq.encode(torch.ones((n, 48), device="cuda"))
+    off = [o and torch.tensor(o, device="cuda") for o in (qo, bo)]
+    bq.grouped_product(q, off[0], b, off[1], out_size=None if bo is None else size)
+    bq.check()
