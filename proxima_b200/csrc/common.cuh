@@ -56,12 +56,16 @@ inline pxc_status ok(pxc_error* err) {
   return PXC_OK;
 }
 
+// The runtime keeps a failed call's error until it is asked for it. It is taken here, or the launch check of a
+// later call would report an allocation that failed before.
 #define PXC_CUDA(expr)                                                                      \
   do {                                                                                      \
     cudaError_t e__ = (expr);                                                               \
-    if (e__ != cudaSuccess)                                                                 \
+    if (e__ != cudaSuccess) {                                                               \
+      cudaGetLastError();                                                                   \
       throw ::pxc::make_failure(PXC_DEVICE, (uint64_t)e__, 0, nullptr, "%s at %s:%d: %s",   \
                                 #expr, __FILE__, __LINE__, cudaGetErrorString(e__));        \
+    }                                                                                       \
   } while (0)
 
 #define PXC_CONFIG(cond, param, value, reason)                                              \

@@ -7,7 +7,7 @@ import pytest
 
 from proxima_b200 import _native as N
 from proxima_b200.blockquant import BlockCodes, BlockQuantizer
-from proxima_b200.errors import Configuration
+from proxima_b200.errors import Configuration, Internal
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -51,3 +51,16 @@ def test_a_products_thread_needs_no_cuda_call_before():
     assert torch.equal(in_a_thread(lambda: bq.encode(bq.decode(q))).codes, q.codes)
     h = BlockCodes(q.codes.cpu().numpy(), q.scales.cpu().numpy(), 48)
     assert np.array_equal(in_a_thread(lambda: bq.product(h, h)), bq.product(q, q).cpu().numpy())
+
+
+def test_a_call_after_one_that_found_no_memory():
+    """300,000 x 300,000 scores are 360 GB, more than the device has; the next call has nothing to do with it."""
+    bq = BlockQuantizer(16)
+    x = torch.ones((3, 16), device="cuda")
+    want = bq.encode(x)
+    h = BlockCodes(np.zeros((300_000, 16), np.uint8), np.zeros((300_000, 4), np.uint8), 16)
+    rows, out = bq._rows(h, False, "h"), np.zeros(16, np.float32)
+    with pytest.raises(Internal):
+        N.call("pxc_bq_product", bq.ctx.handle, C.byref(rows), C.byref(rows), 16, out.ctypes.data, 0, 300_000)
+    got = bq.encode(x)
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
