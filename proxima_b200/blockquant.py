@@ -311,6 +311,9 @@ class BlockQuantizer:
             if not _is_cuda(o) or o.device != dev or o.dtype != _torch().int64 or o.ndim != 1:
                 raise Configuration("offsets", 0, "must be an int64 tensor on the operands' device")
             return o.contiguous()
+        o = np.asarray(o)
+        if o.ndim != 1 or o.dtype.kind not in "iu":
+            raise Configuration("offsets", 0, "must be one row of integers")
         return np.ascontiguousarray(o, np.int64)
 
     def check(self) -> None:

@@ -1,9 +1,24 @@
 """The block quantiser's arguments and handles, as far as no device is needed."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 from proxima_b200 import _native as N
+from proxima_b200.blockquant import BlockCodes, BlockQuantizer
+from proxima_b200.errors import Configuration
+
+
+class NoContext:
+    """Stands for a context: nothing here reaches the device."""
+
+    handle = None
+    device = 0
+
+
+def codes(n, dim):
+    blocks = -(-dim // 128)
+    return BlockCodes(np.zeros((n, -(-dim // 16) * 16), np.uint8), np.zeros((n, -(-blocks // 4) * 4), np.uint8), dim)
 
 
 def test_null_sessions_are_a_status_and_no_crash():
@@ -24,3 +39,16 @@ def test_null_sessions_are_a_status_and_no_crash():
     assert lib.pxc_bq_session_create(None, C.byref(handle), e) == 7 and err.parameter == b"ctx"
     assert handle.value is None
     lib.pxc_bq_session_destroy(None)
+
+
+@pytest.mark.parametrize("bad", [[0, 1.5, 4], [0.0, 4.0], [[0, 1], [1, 4]], np.zeros((2, 0), np.int64), 4, ["0", "4"],
+                                 [False, True]])
+@pytest.mark.parametrize("side", [0, 1])
+def test_host_offsets_that_are_no_row_of_integers_are_refused(bad, side):
+    bq = BlockQuantizer(40, context=NoContext())
+    c = codes(4, 40)
+    good = [0] * (len(bad) - 1) + [4] if np.ndim(bad) else [0, 4]
+    args = [bad, good] if side == 0 else [good, bad]
+    with pytest.raises(Configuration) as e:
+        bq.grouped_product(c, args[0], c, args[1], out_size=16)
+    assert e.value.parameter == "offsets"
