@@ -38,8 +38,23 @@ def _is_cuda(x) -> bool:
     return getattr(x, "is_cuda", False)
 
 
-def _up(x: int, to: int) -> int:
-    return -(-x // to) * to
+def _host_array(x, name: str):
+    """Host rows as an array over the same memory."""
+    if _is_cuda(x):
+        raise Configuration(name, 0, "all operands on one device, or all on the host")
+    if isinstance(x, np.ndarray):
+        return x
+    if str(getattr(x, "dtype", None)) != "torch.uint8":
+        raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
+    return x.numpy()
+
+
+def _host_vectors(x):
+    if hasattr(x, "data_ptr"):
+        x = x.detach()
+        if str(x.dtype) == "torch.bfloat16":  # no such type in NumPy; every value is one in 32 bits
+            x = x.float()
+    return np.asarray(x)
 
 
 def _dtype_code(dtype) -> int:
@@ -154,7 +169,9 @@ class BlockQuantizer:
         if c.dim != self.dim:
             raise DimensionMismatch(self.dim, c.dim)
         codes, scales = c.codes, c.scales
-        if _is_cuda(codes) != cuda or _is_cuda(scales) != cuda:
+        if not cuda:
+            codes, scales = _host_array(codes, name), _host_array(scales, name)
+        elif _is_cuda(codes) != cuda or _is_cuda(scales) != cuda:
             raise Configuration(name, 0, "all operands on one device, or all on the host")
         if codes.ndim != 2 or scales.ndim != 2:
             raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
@@ -184,7 +201,7 @@ class BlockQuantizer:
             if v.ndim == 2 and v.shape[1] == self.dim:
                 return v
         else:
-            v = np.asarray(vectors)
+            v = _host_vectors(vectors)
             if v.dtype not in (np.float32, np.float16):
                 v = v.astype(np.float32)
         if v.ndim == 1 and v.shape[0] % self.dim == 0:
@@ -307,6 +324,8 @@ class BlockQuantizer:
     def _offsets(self, o, cuda: bool, dev):
         if o is None:
             return None
+        if not cuda and _is_cuda(o):
+            raise Configuration("offsets", 0, "all operands on one device, or all on the host")
         if cuda:
             if not _is_cuda(o) or o.device != dev or o.dtype != _torch().int64 or o.ndim != 1:
                 raise Configuration("offsets", 0, "must be an int64 tensor on the operands' device")

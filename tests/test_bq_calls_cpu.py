@@ -52,3 +52,41 @@ def test_host_offsets_that_are_no_row_of_integers_are_refused(bad, side):
     with pytest.raises(Configuration) as e:
         bq.grouped_product(c, args[0], c, args[1], out_size=16)
     assert e.value.parameter == "offsets"
+
+
+class OnDevice:
+    """Stands for a CUDA tensor."""
+
+    is_cuda = True
+    ndim = 2
+
+
+def test_host_tensors_are_taken_or_refused_like_arrays():
+    torch = pytest.importorskip("torch")
+    bq = BlockQuantizer(40, context=NoContext())
+    c = codes(4, 40)
+    t = BlockCodes(torch.from_numpy(c.codes), torch.from_numpy(c.scales), 40)
+    a, b = bq._rows(c, False, "c"), bq._rows(t, False, "t")
+    assert [getattr(a, f) for f, _ in N.PxcBqRows._fields_] == [getattr(b, f) for f, _ in N.PxcBqRows._fields_]
+    for bad in (BlockCodes(t.codes.view(torch.float8_e4m3fn), t.scales, 40), BlockCodes(t.codes.long(), t.scales, 40),
+                BlockCodes(t.codes, c.scales.tolist(), 40), BlockCodes(t.codes, OnDevice(), 40),
+                BlockCodes(t.codes.t(), t.scales, 40), BlockCodes(t.codes[:, ::2], t.scales, 40)):
+        with pytest.raises(Configuration) as e:
+            bq.decode(bad)
+        assert e.value.parameter == "codes"
+        with pytest.raises(Configuration) as e:
+            bq.product(t, bad)
+        assert e.value.parameter == "base"
+    with pytest.raises(Configuration) as e:
+        bq.grouped_product(c, OnDevice(), c)
+    assert e.value.parameter == "offsets"
+
+
+def test_host_vectors_of_any_tensor():
+    torch = pytest.importorskip("torch")
+    bq = BlockQuantizer(40, context=NoContext())
+    x = torch.randn((3, 40), generator=torch.Generator().manual_seed(1))
+    for v in (x, x.half(), x.bfloat16(), x.clone().requires_grad_()):
+        got = bq._vectors(v)
+        assert got.dtype == (np.float16 if v.dtype == torch.float16 else np.float32)
+        assert np.array_equal(got, v.detach().float().numpy())

@@ -64,3 +64,17 @@ def test_a_call_after_one_that_found_no_memory():
         N.call("pxc_bq_product", bq.ctx.handle, C.byref(rows), C.byref(rows), 16, out.ctypes.data, 0, 300_000)
     got = bq.encode(x)
     assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+
+
+def test_host_tensors_give_the_arrays_results():
+    bq = BlockQuantizer(150)
+    x = torch.randn((30, 150), generator=torch.Generator().manual_seed(1))
+    for v in (x, x.half(), x.bfloat16(), x.clone().requires_grad_()):
+        got, want = bq.encode(v), bq.encode(v.detach().cuda())
+        assert isinstance(got.codes, np.ndarray)
+        assert np.array_equal(got.codes, want.codes.cpu().numpy()) and np.array_equal(got.scales, want.scales.cpu().numpy())
+    t = BlockCodes(torch.from_numpy(got.codes), torch.from_numpy(got.scales), 150)
+    assert np.array_equal(bq.decode(t), bq.decode(got))
+    assert np.array_equal(bq.product(t[3:9], t), bq.product(got[3:9], got))
+    off = torch.tensor([0, 9, 30])
+    assert np.array_equal(bq.grouped_product(t, off, t, off), bq.grouped_product(got, off.numpy(), got, off.numpy()))
