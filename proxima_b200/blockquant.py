@@ -60,8 +60,9 @@ def _host_vectors(x):
 def _dtype_code(dtype) -> int:
     code = _codes.get(dtype)
     if code is None:
-        name = str(dtype).split(".")[-1] if "torch" in str(dtype) else np.dtype(dtype).name
-        if name not in _NAMES:
+        tensors = "torch" in str(dtype)
+        name = str(dtype).split(".")[-1] if tensors else np.dtype(dtype).name
+        if name not in _NAMES or not (tensors or np.dtype(dtype).isnative):
             raise Configuration("dtype", 0, f"{name}: must be float32, float16 or bfloat16 (tensors only)")
         code = _codes[dtype] = _NAMES[name]
     return code

@@ -90,3 +90,14 @@ def test_host_vectors_of_any_tensor():
         got = bq._vectors(v)
         assert got.dtype == (np.float16 if v.dtype == torch.float16 else np.float32)
         assert np.array_equal(got, v.detach().float().numpy())
+
+
+@pytest.mark.parametrize("dtype", [">f4", ">f2", np.dtype(np.float16).newbyteorder()])
+def test_results_in_another_byte_order_are_refused(dtype):
+    bq = BlockQuantizer(40, context=NoContext())
+    c = codes(4, 40)
+    for call in (lambda: bq.decode(c, dtype=dtype), lambda: bq.product(c, c, dtype=dtype),
+                 lambda: bq.grouped_product(c, [0, 4], c, dtype=dtype)):
+        with pytest.raises(Configuration) as e:
+            call()
+        assert e.value.parameter == "dtype"
