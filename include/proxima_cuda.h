@@ -768,12 +768,12 @@ uint32_t pxc_sq_last_fallback(const pxc_sq* h);
  * reported once, as PXC_CONFIGURATION ("offsets") or PXC_TIMEOUT, to its own caller
  * and to no other:
  *   - a host form reports its own failure, and nobody else's;
- *   - one of a session's call is reported by a later call of that session;
- *   - one of a device form called with the context itself is reported by a
- *     later such call, or pxc_bq_check, on the same stream; if it was
- *     captured into a graph, on any stream.
+ *   - one of a device form called under a number (pxc_bq_*_as) is reported by a
+ *     later call under that number;
+ *   - one of a device form called without is reported by a later such call, or
+ *     pxc_bq_check, on the same stream; if it was captured into a graph, on any.
  * So callers that share a context and a stream, and run beside one another, take a
- * session each. */
+ * number each. */
 #define PXC_DTYPE_F32 0
 #define PXC_DTYPE_F16 1
 #define PXC_DTYPE_BF16 2
@@ -829,31 +829,31 @@ pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_quer
                                          uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
                                          pxc_error* err);
 /* Waits for `stream` (NULL: the context's) and reports a failure that the device
- * forms called with the context itself left, as above. */
+ * forms left, as above, or callers who were let go of (pxc_bq_forget). */
 pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err);
 
-/* A caller's session: the device forms above, with failures of their own. Creating
- * one may allocate; calls of one session may run concurrently. It may go before
- * its work has run, whose failures nobody is told of then, or after the context. */
-typedef struct pxc_bq_session pxc_bq_session;
-pxc_status pxc_bq_session_create(pxc_ctx* ctx, pxc_bq_session** out, pxc_error* err);
-void pxc_bq_session_destroy(pxc_bq_session* session);
-pxc_status pxc_bq_session_encode(pxc_bq_session* session, const void* d_vectors, int32_t dtype, uint64_t stride,
-                                 uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err);
-pxc_status pxc_bq_session_decode(pxc_bq_session* session, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
-                                 int32_t dtype, uint64_t stride, void* stream, pxc_error* err);
-pxc_status pxc_bq_session_product(pxc_bq_session* session, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
-                                  uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream,
-                                  pxc_error* err);
-pxc_status pxc_bq_session_grouped_product(pxc_bq_session* session, const pxc_bq_rows* d_queries,
-                                          const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
-                                          const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
-                                          int32_t dtype, uint64_t size, void* stream, pxc_error* err);
-/* Reports a failure that is known already, without waiting. */
-pxc_status pxc_bq_session_report(pxc_bq_session* session, pxc_error* err);
-/* Waits for `stream` (NULL: the context's) and reports a failure that the session's
- * calls left, on whichever stream, or that calls with the context itself left on this one. */
-pxc_status pxc_bq_session_check(pxc_bq_session* session, void* stream, pxc_error* err);
+/* The device forms for a caller that names itself by a number (0: as above, told apart by
+ * stream). Its failures are reported to calls with its number alone. */
+/* The first of `count` numbers that this process has not given out before. */
+uint64_t pxc_bq_callers(uint64_t count);
+pxc_status pxc_bq_encode_as(pxc_ctx* ctx, uint64_t caller, const void* d_vectors, int32_t dtype, uint64_t stride,
+                            uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err);
+pxc_status pxc_bq_decode_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
+                            int32_t dtype, uint64_t stride, void* stream, pxc_error* err);
+pxc_status pxc_bq_product_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
+                             uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err);
+pxc_status pxc_bq_grouped_product_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_queries,
+                                     const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
+                                     const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
+                                     int32_t dtype, uint64_t size, void* stream, pxc_error* err);
+/* Reports a failure of the caller's that is known already, without waiting. */
+pxc_status pxc_bq_report_as(pxc_ctx* ctx, uint64_t caller, pxc_error* err);
+/* Waits for `stream` (NULL: the context's) and reports a failure that the caller's calls left, on
+ * whichever stream, that calls without a number left on this one, or that callers left who were let go of. */
+pxc_status pxc_bq_check_as(pxc_ctx* ctx, uint64_t caller, void* stream, pxc_error* err);
+/* Lets go of what is kept for these callers, who make no further calls. Their work may still run; its
+ * failures are reported by any later check. */
+pxc_status pxc_bq_forget(pxc_ctx* ctx, const uint64_t* callers, uint64_t count, pxc_error* err);
 
 #ifdef __cplusplus
 }

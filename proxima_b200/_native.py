@@ -281,18 +281,19 @@ SIGNATURES: dict[str, tuple] = {
     "pxc_bq_grouped_product_device": (C.c_int32, [vp, C.POINTER(PxcBqRows), vp, C.POINTER(PxcBqRows), vp, C.c_uint32,
                                                   C.c_uint32, vp, C.c_int32, C.c_uint64, vp, C.POINTER(PxcError)]),
     "pxc_bq_check": (C.c_int32, [vp, vp, C.POINTER(PxcError)]),
-    "pxc_bq_session_create": (C.c_int32, [vp, C.POINTER(vp), C.POINTER(PxcError)]),
-    "pxc_bq_session_destroy": (None, [vp]),
-    "pxc_bq_session_encode": (C.c_int32, [vp, vp, C.c_int32, C.c_uint64, C.c_uint32, C.POINTER(PxcBqRows), vp,
-                                          C.POINTER(PxcError)]),
-    "pxc_bq_session_decode": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32, C.c_uint64, vp,
-                                          C.POINTER(PxcError)]),
-    "pxc_bq_session_product": (C.c_int32, [vp, C.POINTER(PxcBqRows), C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32,
-                                           C.c_uint64, vp, C.POINTER(PxcError)]),
-    "pxc_bq_session_grouped_product": (C.c_int32, [vp, C.POINTER(PxcBqRows), vp, C.POINTER(PxcBqRows), vp, C.c_uint32,
-                                                   C.c_uint32, vp, C.c_int32, C.c_uint64, vp, C.POINTER(PxcError)]),
-    "pxc_bq_session_report": (C.c_int32, [vp, C.POINTER(PxcError)]),
-    "pxc_bq_session_check": (C.c_int32, [vp, vp, C.POINTER(PxcError)]),
+    "pxc_bq_callers": (C.c_uint64, [C.c_uint64]),
+    "pxc_bq_encode_as": (C.c_int32, [vp, C.c_uint64, vp, C.c_int32, C.c_uint64, C.c_uint32, C.POINTER(PxcBqRows), vp,
+                                     C.POINTER(PxcError)]),
+    "pxc_bq_decode_as": (C.c_int32, [vp, C.c_uint64, C.POINTER(PxcBqRows), C.c_uint32, vp, C.c_int32, C.c_uint64, vp,
+                                     C.POINTER(PxcError)]),
+    "pxc_bq_product_as": (C.c_int32, [vp, C.c_uint64, C.POINTER(PxcBqRows), C.POINTER(PxcBqRows), C.c_uint32, vp,
+                                      C.c_int32, C.c_uint64, vp, C.POINTER(PxcError)]),
+    "pxc_bq_grouped_product_as": (C.c_int32, [vp, C.c_uint64, C.POINTER(PxcBqRows), vp, C.POINTER(PxcBqRows), vp,
+                                              C.c_uint32, C.c_uint32, vp, C.c_int32, C.c_uint64, vp,
+                                              C.POINTER(PxcError)]),
+    "pxc_bq_report_as": (C.c_int32, [vp, C.c_uint64, C.POINTER(PxcError)]),
+    "pxc_bq_check_as": (C.c_int32, [vp, C.c_uint64, vp, C.POINTER(PxcError)]),
+    "pxc_bq_forget": (C.c_int32, [vp, C.POINTER(C.c_uint64), C.c_uint64, C.POINTER(PxcError)]),
 }
 
 _lib = None

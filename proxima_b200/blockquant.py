@@ -15,12 +15,13 @@ rows, or the tokens of an expert with the expert's weights.
 
 CUDA tensors in give CUDA tensors out, computed on the current stream without a wait; a
 failure that only the device sees (bad offsets) is raised by a later call of the same quantiser, or by its
-``check()``, and by nobody else's: callers in several threads have a quantiser each. Host arrays in give NumPy arrays out. There is no CPU path.
+``check()``, and by no other quantiser's: callers in several threads have one each. Of a quantiser that
+is gone, any ``check()`` raises it. Host arrays in give NumPy arrays out. There is no CPU path.
 """
 from __future__ import annotations
 
 import ctypes as C
-import threading
+import itertools
 from dataclasses import dataclass
 from typing import Any
 
@@ -32,6 +33,14 @@ from .errors import Configuration, DimensionMismatch
 BLOCK = 128
 _NAMES = {"float32": 0, "float16": 1, "bfloat16": 2}
 _codes: dict = {}  # dtype -> its code, torch's types among them once torch is in use
+_numbers = None  # the numbers under which quantisers make their calls
+
+
+def _count():
+    global _numbers
+    if _numbers is None:
+        _numbers = itertools.count(N.load().pxc_bq_callers(1 << 48))
+    return _numbers
 
 
 def _is_cuda(x) -> bool:
@@ -77,8 +86,8 @@ class _Torch:
         self.uint8, self.int64, self.float32, self.empty = torch.uint8, torch.int64, torch.float32, torch.empty
         self.current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
-        self.encode, self.decode = N.bind("pxc_bq_session_encode"), N.bind("pxc_bq_session_decode")
-        self.product, self.grouped = N.bind("pxc_bq_session_product"), N.bind("pxc_bq_session_grouped_product")
+        self.encode, self.decode = N.bind("pxc_bq_encode_as"), N.bind("pxc_bq_decode_as")
+        self.product, self.grouped = N.bind("pxc_bq_product_as"), N.bind("pxc_bq_grouped_product_as")
 
 
 _torch_parts: _Torch | None = None
@@ -89,21 +98,6 @@ def _torch() -> _Torch:
     if _torch_parts is None:
         _torch_parts = _Torch()
     return _torch_parts
-
-
-class _Session:
-    """The native record of a quantiser's failures (pxc_bq_session)."""
-
-    def __init__(self, context):
-        handle = N.vp()
-        N.call("pxc_bq_session_create", context.handle, C.byref(handle))
-        self.handle = handle.value
-
-    def __del__(self):
-        try:
-            N.load().pxc_bq_session_destroy(self.handle)
-        except Exception:
-            pass
 
 
 @dataclass(slots=True)
@@ -143,27 +137,41 @@ class BlockQuantizer:
         self.ctx = context
         self.blocks = -(-dim // BLOCK)
         self._ld, self._sld = (dim + 15) & ~15, (self.blocks + 3) & ~3
-        self._session = None
-        self._opening = threading.Lock()
+        self._caller = next(_numbers or _count())
+        try:  # quantisers of the context that are gone, until the native side is told
+            self._gone = context._gone_callers
+        except AttributeError:
+            self._gone = context._gone_callers = []
 
-    def _open(self) -> _Session:
-        with self._opening:
-            if self._session is None:
-                self._session = _Session(self.ctx)
-        return self._session
+    def __del__(self):
+        try:
+            self._gone.append(self._caller)
+            if len(self._gone) >= 64:
+                self._forget()
+        except Exception:
+            pass
+
+    def _forget(self) -> None:
+        gone = []
+        try:
+            while True:  # others may be at it too
+                gone.append(self._gone.pop())
+        except IndexError:
+            pass
+        N.call("pxc_bq_forget", self.ctx.handle, (C.c_uint64 * len(gone))(*gone), len(gone))
 
     def _host(self, name: str, *args) -> None:
         """A host form, which reports its own failure; what tensors' calls left is raised first."""
-        N.call("pxc_bq_session_report", (self._session or self._open()).handle)
+        N.call("pxc_bq_report_as", self.ctx.handle, self._caller)
         N.call(name, self.ctx.handle, *args)
 
     # -- arguments --
-    def _stream(self, tensor) -> int:
+    def _stream(self, t: _Torch, tensor) -> int:
         """The current stream of the tensor's device; 1 names the legacy default stream."""
         index = tensor.get_device()
         if index != self.ctx.device:
             raise Configuration("device", index, f"the context is on device {self.ctx.device}")
-        return _torch().current_stream(index) or 1
+        return t.current_stream(index) or 1
 
     def _rows(self, c: BlockCodes, cuda: bool, name: str) -> N.PxcBqRows:
         """The rows as the native calls take them: tensors on the context's device, or arrays."""
@@ -222,7 +230,7 @@ class BlockQuantizer:
             code = _codes.get(v.dtype)
             if code is None:
                 code = _dtype_code(v.dtype)
-            stream = self._stream(v)
+            stream = self._stream(t, v)
             row, step = v.stride()
             if (step != 1 and dim > 1) or (row < dim and n > 1):
                 v = v.contiguous()
@@ -230,7 +238,7 @@ class BlockQuantizer:
             codes = t.empty(n, ld, dtype=t.uint8, device=v.device)
             scales = codes.new_empty(n, sld)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
-            t.encode((self._session or self._open()).handle, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
+            t.encode(self.ctx.handle, self._caller, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
             return BlockCodes(codes, scales, dim)
         v = np.ascontiguousarray(v)
         codes, scales = np.zeros((n, ld), np.uint8), np.zeros((n, sld), np.uint8)
@@ -244,10 +252,13 @@ class BlockQuantizer:
         rows = self._rows(codes, cuda, "codes")
         if cuda:
             t = _torch()
-            code = _dtype_code(dtype or t.float32)
-            out = t.empty(rows.rows, self.dim, dtype=dtype or t.float32, device=codes.codes.device)
-            t.decode((self._session or self._open()).handle, C.byref(rows), self.dim, out.data_ptr(), code, self.dim,
-                     self._stream(out))
+            dtype = dtype or t.float32
+            code = _codes.get(dtype)
+            if code is None:
+                code = _dtype_code(dtype)
+            out = t.empty(rows.rows, self.dim, dtype=dtype, device=codes.codes.device)
+            t.decode(self.ctx.handle, self._caller, C.byref(rows), self.dim, out.data_ptr(), code, self.dim,
+                     self._stream(t, out))
             return out
         out = np.zeros((len(codes), self.dim), dtype or np.float32)
         self._host("pxc_bq_decode", C.byref(rows), self.dim, N.ptr(out), _dtype_code(out.dtype), self.dim)
@@ -264,16 +275,19 @@ class BlockQuantizer:
             t, dev = _torch(), queries.codes.device
             stride = shape[1] or 1
             if out is None:
-                code = _dtype_code(dtype or t.float32)
-                out = t.empty(*shape, dtype=dtype or t.float32, device=dev)
+                dtype = dtype or t.float32
+                code = _codes.get(dtype)
+                if code is None:
+                    code = _dtype_code(dtype)
+                out = t.empty(*shape, dtype=dtype, device=dev)
             else:
                 if (tuple(out.shape) != shape or out.device != dev or (dtype is not None and out.dtype != dtype)
                         or (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1])):
                     raise Configuration("out", 0, "must be (nq, n) on the operands' device, with contiguous rows")
                 code = _dtype_code(out.dtype)
                 stride = out.stride(0) if shape[0] > 1 else stride
-            t.product((self._session or self._open()).handle, C.byref(q), C.byref(b), self.dim, out.data_ptr(), code,
-                      stride, self._stream(out))
+            t.product(self.ctx.handle, self._caller, C.byref(q), C.byref(b), self.dim, out.data_ptr(), code,
+                      stride, self._stream(t, out))
             return out
         if out is not None:
             raise Configuration("out", 0, "is for tensors")
@@ -312,10 +326,13 @@ class BlockQuantizer:
             shape = (size,)
         if cuda:
             t = _torch()
-            code = _dtype_code(dtype or t.float32)
-            out = t.empty(*shape, dtype=dtype or t.float32, device=dev)
-            t.grouped((self._session or self._open()).handle, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups,
-                      self.dim, out.data_ptr(), code, size, self._stream(out))
+            dtype = dtype or t.float32
+            code = _codes.get(dtype)
+            if code is None:
+                code = _dtype_code(dtype)
+            out = t.empty(*shape, dtype=dtype, device=dev)
+            t.grouped(self.ctx.handle, self._caller, C.byref(q), qo.data_ptr(), C.byref(b), N.ptr(bo), groups,
+                      self.dim, out.data_ptr(), code, size, self._stream(t, out))
             return out
         out = np.zeros(shape, dtype or np.float32)
         self._host("pxc_bq_grouped_product", C.byref(q), N.ptr(qo), C.byref(b), N.ptr(bo), groups, self.dim,
@@ -338,6 +355,7 @@ class BlockQuantizer:
 
     def check(self) -> None:
         """Waits for the current stream and raises a failure that an earlier call of this quantiser left on the
-        device, or one that calls of the C functions with its context left on this stream."""
-        session = self._session or self._open()
-        N.call("pxc_bq_session_check", session.handle, _torch().current_stream(self.ctx.device) or 1)
+        device; or one of quantisers that are gone, or of C functions called without a caller's number on this stream."""
+        if self._gone:
+            self._forget()
+        N.call("pxc_bq_check_as", self.ctx.handle, self._caller, _torch().current_stream(self.ctx.device) or 1)

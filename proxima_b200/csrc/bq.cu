@@ -1,7 +1,6 @@
 // bq.cu — the block quantiser (pxc_bq_*): encode, decode, the product of two sets of
 // encoded rows, and the product grouped by ragged lists.
 #include <algorithm>
-#include <memory>
 #include <type_traits>
 
 #include "bq.cuh"
@@ -387,10 +386,15 @@ struct Caller {
   Record record;    // what this call's kernels write
   Record told[2];   // earlier failures that the call reports
 
-  Caller(pxc_ctx* c, void* s) : ctx(c) {
+  // `number` 0: told apart by stream. `fails`: this call may leave a failure.
+  Caller(pxc_ctx* c, uint64_t number, void* s, bool fails) : ctx(c) {
     PXC_CONFIG(ctx != nullptr, "ctx", 0, "null context");
     stream = s ? static_cast<cudaStream_t>(s) : ctx->stream;
     Reports& reports = *ctx->bq_reports;
+    if (number != 0) {
+      told[0] = record = reports.of_caller(number, fails);
+      return;
+    }
     told[0] = record = reports.of_stream(stream);
     told[1] = reports.captured();
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -398,13 +402,6 @@ struct Caller {
       cudaGetLastError();  // the launch will say what is wrong
     else if (status != cudaStreamCaptureStatusNone)
       record = reports.captured();
-  }
-  Caller(pxc_bq_session* session, void* s) {
-    PXC_CONFIG(session != nullptr, "session", 0, "null session");
-    ctx = session->reports->context();
-    PXC_CONFIG(ctx != nullptr, "ctx", 0, "the session's context has gone");
-    stream = s ? static_cast<cudaStream_t>(s) : ctx->stream;
-    told[0] = record = session->record;
   }
   void report() const {
     for (const Record& r : told)
@@ -699,7 +696,7 @@ static void check_host_offsets(const int64_t* o, uint32_t groups, uint64_t rows)
                "offsets must rise and stay within the rows");
 }
 
-// ---- the device forms, of a context's or a session's caller ----
+// ---- the device forms ----
 static void encode_device(const Caller& c, const void* vectors, int32_t dtype, uint64_t stride, uint32_t dim,
                           const pxc_bq_rows* out) {
   check_common(dim, dtype);
@@ -774,7 +771,7 @@ extern "C" {
 pxc_status pxc_bq_encode_device(pxc_ctx* ctx, const void* d_vectors, int32_t dtype, uint64_t stride, uint32_t dim,
                                 const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::encode_device(bq::Caller(ctx, stream), d_vectors, dtype, stride, dim, d_out);
+    bq::encode_device(bq::Caller(ctx, 0, stream, false), d_vectors, dtype, stride, dim, d_out);
   });
 }
 
@@ -805,7 +802,7 @@ pxc_status pxc_bq_encode(pxc_ctx* ctx, const void* vectors, int32_t dtype, uint6
 pxc_status pxc_bq_decode_device(pxc_ctx* ctx, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out, int32_t dtype,
                                 uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::decode_device(bq::Caller(ctx, stream), d_rows, dim, d_out, dtype, stride);
+    bq::decode_device(bq::Caller(ctx, 0, stream, false), d_rows, dim, d_out, dtype, stride);
   });
 }
 
@@ -834,7 +831,7 @@ pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, vo
 pxc_status pxc_bq_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base, uint32_t dim,
                                  void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::product_device(bq::Caller(ctx, stream), d_queries, d_base, dim, d_out, dtype, stride);
+    bq::product_device(bq::Caller(ctx, 0, stream, true), d_queries, d_base, dim, d_out, dtype, stride);
   });
 }
 
@@ -870,7 +867,7 @@ pxc_status pxc_bq_grouped_product_device(pxc_ctx* ctx, const pxc_bq_rows* d_quer
                                          uint32_t dim, void* d_out, int32_t dtype, uint64_t size, void* stream,
                                          pxc_error* err) {
   return guarded(err, [&] {
-    bq::grouped_device(bq::Caller(ctx, stream), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim, d_out,
+    bq::grouped_device(bq::Caller(ctx, 0, stream, true), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim, d_out,
                        dtype, size);
   });
 }
@@ -927,75 +924,64 @@ pxc_status pxc_bq_grouped_product(pxc_ctx* ctx, const pxc_bq_rows* queries, cons
   });
 }
 
-pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err) {
-  return guarded(err, [&] {
-    const bq::Caller c(ctx, stream);
-    DeviceGuard g(ctx->device);
-    PXC_CUDA(cudaStreamSynchronize(c.stream));
-    c.report();
-  });
+pxc_status pxc_bq_check(pxc_ctx* ctx, void* stream, pxc_error* err) { return pxc_bq_check_as(ctx, 0, stream, err); }
+
+uint64_t pxc_bq_callers(uint64_t count) {
+  static uint64_t next = 1;
+  return __atomic_fetch_add(&next, count, __ATOMIC_RELAXED);
 }
 
-pxc_status pxc_bq_session_create(pxc_ctx* ctx, pxc_bq_session** out, pxc_error* err) {
+pxc_status pxc_bq_forget(pxc_ctx* ctx, const uint64_t* callers, uint64_t count, pxc_error* err) {
   return guarded(err, [&] {
     bq::check_context(ctx);
-    PXC_CONFIG(out != nullptr, "out", 0, "null output");
-    auto h = std::make_unique<pxc_bq_session>();
-    h->reports = ctx->bq_reports;
-    h->record = h->reports->lease();
-    *out = h.release();
+    PXC_CONFIG(callers != nullptr || count == 0, "callers", 0, "null callers");
+    ctx->bq_reports->forget(callers, count);
   });
 }
 
-void pxc_bq_session_destroy(pxc_bq_session* session) {
-  if (!session) return;
-  session->reports->give_back(session->record);
-  delete session;
-}
-
-pxc_status pxc_bq_session_encode(pxc_bq_session* session, const void* d_vectors, int32_t dtype, uint64_t stride,
-                                 uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
+pxc_status pxc_bq_encode_as(pxc_ctx* ctx, uint64_t caller, const void* d_vectors, int32_t dtype, uint64_t stride,
+                            uint32_t dim, const pxc_bq_rows* d_out, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::encode_device(bq::Caller(session, stream), d_vectors, dtype, stride, dim, d_out);
+    bq::encode_device(bq::Caller(ctx, caller, stream, false), d_vectors, dtype, stride, dim, d_out);
   });
 }
 
-pxc_status pxc_bq_session_decode(pxc_bq_session* session, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
-                                 int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
+pxc_status pxc_bq_decode_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out,
+                            int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::decode_device(bq::Caller(session, stream), d_rows, dim, d_out, dtype, stride);
+    bq::decode_device(bq::Caller(ctx, caller, stream, false), d_rows, dim, d_out, dtype, stride);
   });
 }
 
-pxc_status pxc_bq_session_product(pxc_bq_session* session, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
-                                  uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream,
-                                  pxc_error* err) {
+pxc_status pxc_bq_product_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_queries, const pxc_bq_rows* d_base,
+                             uint32_t dim, void* d_out, int32_t dtype, uint64_t stride, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::product_device(bq::Caller(session, stream), d_queries, d_base, dim, d_out, dtype, stride);
+    bq::product_device(bq::Caller(ctx, caller, stream, true), d_queries, d_base, dim, d_out, dtype, stride);
   });
 }
 
-pxc_status pxc_bq_session_grouped_product(pxc_bq_session* session, const pxc_bq_rows* d_queries,
-                                          const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
-                                          const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
-                                          int32_t dtype, uint64_t size, void* stream, pxc_error* err) {
+pxc_status pxc_bq_grouped_product_as(pxc_ctx* ctx, uint64_t caller, const pxc_bq_rows* d_queries,
+                                     const int64_t* d_query_offsets, const pxc_bq_rows* d_base,
+                                     const int64_t* d_base_offsets, uint32_t groups, uint32_t dim, void* d_out,
+                                     int32_t dtype, uint64_t size, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    bq::grouped_device(bq::Caller(session, stream), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim,
+    bq::grouped_device(bq::Caller(ctx, caller, stream, true), d_queries, d_query_offsets, d_base, d_base_offsets, groups, dim,
                        d_out, dtype, size);
   });
 }
 
-pxc_status pxc_bq_session_report(pxc_bq_session* session, pxc_error* err) {
-  return guarded(err, [&] { bq::Caller(session, nullptr).report(); });
+pxc_status pxc_bq_report_as(pxc_ctx* ctx, uint64_t caller, pxc_error* err) {
+  return guarded(err, [&] { bq::Caller(ctx, caller, nullptr, false).report(); });
 }
 
-pxc_status pxc_bq_session_check(pxc_bq_session* session, void* stream, pxc_error* err) {
+pxc_status pxc_bq_check_as(pxc_ctx* ctx, uint64_t caller, void* stream, pxc_error* err) {
   return guarded(err, [&] {
-    const bq::Caller c(session, stream);
-    DeviceGuard g(c.ctx->device);
+    const bq::Caller c(ctx, caller, stream, false);
+    DeviceGuard g(ctx->device);
     PXC_CUDA(cudaStreamSynchronize(c.stream));
     c.report();
-    c.ctx->bq_reports->of_stream(c.stream).take();
+    if (caller != 0) ctx->bq_reports->of_stream(c.stream).take();
+    ctx->bq_reports->take_left();
   });
 }
 

@@ -1,14 +1,13 @@
 // bq_reports.cuh — failures of block products that only the device sees, kept apart by caller.
 //
-// A caller has a record: two words of pinned host memory that its calls' kernels write, and a number that they
-// write into them. Callers are the sessions, the streams of calls made with the context itself, and
-// each host call. Numbers are never used twice, so a kernel or graph that outlives its caller tells nobody
-// else, and the words stay allocated until the context goes. They are given out again late: behind at
-// least QUARANTINE others.
+// A caller has a record: two words of pinned host memory that its calls' kernels write, and an id that they
+// write into them. Callers are those that name themselves by a number, the streams of calls made without one, and
+// each host call. Ids are never used twice, so a kernel or graph that outlives its caller is not taken for
+// another's, and the words stay allocated until the context goes. A record whose caller has gone is given out again
+// late, behind at least QUARANTINE others; what its work leaves meanwhile is for whoever checks.
 #pragma once
 
 #include <deque>
-#include <memory>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -25,37 +24,33 @@ struct Record {
   uint32_t* words = nullptr;
   uint32_t id = 0;
 
+  // Whether a failure of this kind is there; it is so once.
+  bool taken(Fault f) const {
+    uint32_t seen = __atomic_load_n(words + f, __ATOMIC_RELAXED);
+    return seen == id && id != 0 &&
+           __atomic_compare_exchange_n(words + f, &seen, 0u, false, __ATOMIC_RELAXED, __ATOMIC_RELAXED);
+  }
   // Reports a failure, once. Of two kinds, the other stays for the next call.
   void take() const {
-    for (const Fault f : {FAULT_TIMEOUT, FAULT_OFFSETS}) {
-      uint32_t seen = __atomic_load_n(words + f, __ATOMIC_RELAXED);
-      if (seen != id || !__atomic_compare_exchange_n(words + f, &seen, 0u, false, __ATOMIC_RELAXED, __ATOMIC_RELAXED))
-        continue;
-      if (f == FAULT_TIMEOUT)
-        throw make_failure(PXC_TIMEOUT, 0, 0, nullptr, "a device-side wait of a block product ran out");
-      throw make_failure(PXC_CONFIGURATION, 0, 0, "offsets",
-                         "a grouped product's offsets fell, left the rows, or did not fit the output");
-    }
+    for (const Fault f : {FAULT_TIMEOUT, FAULT_OFFSETS})
+      if (taken(f)) raise(f);
+  }
+  [[noreturn]] static void raise(Fault f) {
+    if (f == FAULT_TIMEOUT)
+      throw make_failure(PXC_TIMEOUT, 0, 0, nullptr, "a device-side wait of a block product ran out");
+    throw make_failure(PXC_CONFIGURATION, 0, 0, "offsets",
+                       "a grouped product's offsets fell, left the rows, or did not fit the output");
   }
 };
 
 class Reports {
  public:
-  explicit Reports(pxc_ctx* ctx) : ctx_(ctx) { add_slab(); }
-  ~Reports() { close(); }
+  explicit Reports(int device) : device_(device) { add_slab(); }
+  ~Reports() {
+    for (uint32_t* s : slabs_) cudaFreeHost(s);
+  }
   Reports(const Reports&) = delete;
   Reports& operator=(const Reports&) = delete;
-
-  // NULL once the context has gone; sessions may outlive it.
-  pxc_ctx* context() const { return __atomic_load_n(&ctx_, __ATOMIC_ACQUIRE); }
-
-  void close() {
-    std::lock_guard<std::mutex> lock(mu_);
-    __atomic_store_n(&ctx_, static_cast<pxc_ctx*>(nullptr), __ATOMIC_RELEASE);
-    for (uint32_t* s : slabs_) cudaFreeHost(s);
-    slabs_.clear();
-    free_.clear();
-  }
 
   Record lease() {
     std::lock_guard<std::mutex> lock(mu_);
@@ -65,12 +60,41 @@ class Reports {
   void give_back(const Record& r) noexcept {
     try {
       std::lock_guard<std::mutex> lock(mu_);
-      if (!slabs_.empty()) free_.push_back(r.words);
+      free_.push_back(Record{r.words, 0});
     } catch (...) {  // no memory for the list: this one stays out of it
     }
   }
 
-  // The record of calls made with the context on `s`, and the one that all its captured calls share: on which
+  // The record of a caller's number. Without `make`, an empty one where no call has needed it yet.
+  Record of_caller(uint64_t caller, bool make) {
+    std::lock_guard<std::mutex> lock(mu_);
+    const auto found = callers_.find(caller);
+    if (found != callers_.end()) return found->second;
+    if (!make) return Record{};
+    Record& r = callers_[caller];
+    return r = take_slot();
+  }
+  void forget(const uint64_t* callers, uint64_t count) {
+    std::lock_guard<std::mutex> lock(mu_);
+    for (uint64_t i = 0; i < count; ++i) {
+      const auto found = callers_.find(callers[i]);
+      if (found == callers_.end()) continue;
+      free_.push_back(found->second);
+      callers_.erase(found);
+    }
+  }
+  // Reports a failure that the work of a caller left who has gone.
+  void take_left() {
+    std::lock_guard<std::mutex> lock(mu_);
+    for (const Record& r : free_) r.take();
+    for (const Fault f : {FAULT_TIMEOUT, FAULT_OFFSETS})
+      if (left_[f]) {
+        left_[f] = false;
+        Record::raise(f);
+      }
+  }
+
+  // The record of calls without a number on `s`, and the one that all such captured calls share: on which
   // stream a graph runs is not known when it is captured.
   Record of_stream(cudaStream_t s) {
     static thread_local char thread;  // the per-thread default stream is another one in each thread
@@ -86,16 +110,16 @@ class Reports {
 
   Record take_slot() {
     if (free_.size() <= QUARANTINE) add_slab();
-    Record r;
-    r.words = free_.front();
+    Record r = free_.front();
     free_.pop_front();
+    for (const Fault f : {FAULT_TIMEOUT, FAULT_OFFSETS}) left_[f] = r.taken(f) || left_[f];
     if (++last_id_ == 0) ++last_id_;
     r.id = last_id_;
     return r;
   }
 
   void add_slab() {
-    DeviceGuard g(ctx_->device);
+    DeviceGuard g(device_);
     // allocating must not disturb a capture that is under way in this thread
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     PXC_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
@@ -105,14 +129,16 @@ class Reports {
     PXC_CUDA(e);
     slabs_.push_back(s);
     std::memset(s, 0, SLAB * FAULT_WORDS * sizeof(uint32_t));
-    for (size_t i = 0; i < SLAB; ++i) free_.push_back(s + i * FAULT_WORDS);
+    for (size_t i = 0; i < SLAB; ++i) free_.push_back(Record{s + i * FAULT_WORDS, 0});
     if (!captured_.words) captured_ = take_slot();
   }
 
-  pxc_ctx* ctx_;
+  const int device_;
   std::mutex mu_;
   std::vector<uint32_t*> slabs_;
-  std::deque<uint32_t*> free_;
+  std::deque<Record> free_;  // with the ids of callers who have gone
+  bool left_[FAULT_WORDS] = {};  // failures found in a record that was given out again
+  std::unordered_map<uint64_t, Record> callers_;
   std::unordered_map<const void*, Record> streams_;
   Record captured_;
   uint32_t last_id_ = 0;
@@ -128,8 +154,3 @@ struct Leased {
 
 }  // namespace bq
 }  // namespace pxc
-
-struct pxc_bq_session {
-  std::shared_ptr<pxc::bq::Reports> reports;
-  pxc::bq::Record record;
-};

@@ -144,7 +144,7 @@ struct pxc_ctx {
   uint32_t wait_ms = 2000;
   uint32_t* d_status = nullptr;  // [0] device error word, [1] aux
   uint32_t* h_status = nullptr;  // pinned mirror
-  std::shared_ptr<pxc::bq::Reports> bq_reports;  // failures of block products (bq_reports.cuh)
+  std::shared_ptr<pxc::bq::Reports> bq_reports;  // failures of block products, by caller (bq_reports.cuh)
   uint32_t bq_ready = 0;          // block product kernels (a bit each) set up on the device
   int sm_count = 0;
   bool profiling = false;

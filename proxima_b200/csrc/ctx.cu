@@ -380,7 +380,7 @@ pxc_status pxc_ctx_create(const int* devices, int n_devices, pxc_ctx** out, pxc_
       PXC_CUDA(cudaMalloc(&c->d_status, 2 * sizeof(uint32_t)));
       PXC_CUDA(cudaMemset(c->d_status, 0, 2 * sizeof(uint32_t)));
       PXC_CUDA(cudaMallocHost(&c->h_status, 2 * sizeof(uint32_t)));
-      c->bq_reports = std::make_shared<bq::Reports>(c);
+      c->bq_reports = std::make_shared<bq::Reports>(dev);
     } catch (...) {
       pxc_ctx_destroy(c);
       throw;
@@ -405,7 +405,7 @@ void pxc_ctx_destroy(pxc_ctx* ctx) {
   if (ctx->crc_host) cudaFreeHost(ctx->crc_host);
   if (ctx->d_status) cudaFree(ctx->d_status);
   if (ctx->h_status) cudaFreeHost(ctx->h_status);
-  if (ctx->bq_reports) ctx->bq_reports->close();
+  ctx->bq_reports.reset();
   if (ctx->stream) cudaStreamDestroy(ctx->stream);
   if (prev >= 0) cudaSetDevice(prev);
   delete ctx;

@@ -21,24 +21,29 @@ def codes(n, dim):
     return BlockCodes(np.zeros((n, -(-dim // 16) * 16), np.uint8), np.zeros((n, -(-blocks // 4) * 4), np.uint8), dim)
 
 
-def test_null_sessions_are_a_status_and_no_crash():
+def test_null_contexts_are_a_status_and_no_crash():
     lib = N.load()
     rows = N.PxcBqRows(None, None, 0, 16, 4)
     err = N.PxcError()
     r, e = C.byref(rows), C.byref(err)
     for status in (
-        lib.pxc_bq_session_encode(None, None, 0, 8, 8, r, None, e),
-        lib.pxc_bq_session_decode(None, r, 8, None, 0, 8, None, e),
-        lib.pxc_bq_session_product(None, r, r, 8, None, 0, 8, None, e),
-        lib.pxc_bq_session_grouped_product(None, r, None, r, None, 1, 8, None, 0, 0, None, e),
-        lib.pxc_bq_session_report(None, e),
-        lib.pxc_bq_session_check(None, None, e),
+        lib.pxc_bq_encode_as(None, 7, None, 0, 8, 8, r, None, e),
+        lib.pxc_bq_decode_as(None, 7, r, 8, None, 0, 8, None, e),
+        lib.pxc_bq_product_as(None, 7, r, r, 8, None, 0, 8, None, e),
+        lib.pxc_bq_grouped_product_as(None, 7, r, None, r, None, 1, 8, None, 0, 0, None, e),
+        lib.pxc_bq_report_as(None, 7, e),
+        lib.pxc_bq_check_as(None, 7, None, e),
+        lib.pxc_bq_forget(None, None, 0, e),
     ):
-        assert status == 7 and err.parameter == b"session"
-    handle = N.vp()
-    assert lib.pxc_bq_session_create(None, C.byref(handle), e) == 7 and err.parameter == b"ctx"
-    assert handle.value is None
-    lib.pxc_bq_session_destroy(None)
+        assert status == 7 and err.parameter == b"ctx"
+
+
+def test_callers_numbers_are_given_out_once():
+    lib = N.load()
+    a, b, c = lib.pxc_bq_callers(5), lib.pxc_bq_callers(1), lib.pxc_bq_callers(1)
+    assert a > 0 and b == a + 5 and c == b + 1
+    own = [BlockQuantizer(40, context=NoContext())._caller for _ in range(100)]
+    assert len(set(own)) == 100
 
 
 @pytest.mark.parametrize("bad", [[0, 1.5, 4], [0.0, 4.0], [[0, 1], [1, 4]], np.zeros((2, 0), np.int64), 4, ["0", "4"],

@@ -255,26 +255,38 @@ def test_graphs_report_to_the_quantiser_that_was_captured(ctx):
         a.product(q, base)
 
 
-def test_quantisers_that_come_and_go(ctx):
-    """A quantiser may go before its work has run; nobody else is told of it, and there are many."""
-    first = BlockQuantizer(48, context=ctx)
-    q, base = some_codes(first, 20, 1), some_codes(first, 40, 2)
-    want = first.product(q, base)
-    kept = []
+def test_failures_of_quantisers_that_are_gone(ctx):
+    """Their work may still run. No other quantiser's calls are told of it, but whoever checks is."""
+    kept = BlockQuantizer(48, context=ctx)
+    q, base = some_codes(kept, 20, 1), some_codes(kept, 40, 2)
+    want = kept.product(q, base)
     for i in range(3000):
         bad_call(BlockQuantizer(48, context=ctx), q, base)
-        later = BlockQuantizer(48, context=ctx)
         if i % 100 == 0:
-            assert torch.equal(later.product(q, base), want)
-            kept.append(later)
-    for k in kept:
-        k.check()
-    first.check()
-    bad_call(kept[3], q, base)
-    for k in kept[:3] + kept[4:]:
-        k.check()
+            later = BlockQuantizer(48, context=ctx)
+            assert torch.equal(later.product(q, base), want) and torch.equal(kept.product(q, base), want)
+    told = 0
+    for _ in range(3001):
+        try:
+            BlockQuantizer(48, context=ctx).check()
+            break
+        except Configuration:
+            told += 1
+    assert 1 <= told <= 3000
+    kept.check()
+    # a graph that outlives the quantiser it was captured with
+    off = torch.tensor([0, 10, 20], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        BlockQuantizer(48, context=ctx).grouped_product(q, off, base)
+    off.copy_(torch.tensor(BAD))
+    kept.check()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(kept.product(q, base), want)
     with pytest.raises(Configuration):
-        kept[3].check()
+        kept.check()
+    kept.check()
 
 
 def test_a_closed_context_is_refused():
