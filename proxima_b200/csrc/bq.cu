@@ -568,11 +568,15 @@ static void product(pxc_ctx* ctx, const pxc_bq_rows& q, const pxc_bq_rows& b, ui
     pair = shape.pair;
     p.subs = q.rows <= shape.width && !pair ? narrow_subs(p.q_rows, b.rows, ctx->sm_count) : 1;
   } else {
-    // room for twice the mean, so that most groups are one tile and the rings stay deep; pairs where the mean
-    // fills them (8192 queries over 32 groups: 45 us, without 46; over 500 lists of 40: 47 us, without 44)
+    // room for twice the mean, so that most groups are one tile and the rings stay deep
     const uint64_t mean = q.rows / g.groups;
     p.tile_q = p.q_rows = static_cast<uint32_t>(std::min<uint64_t>(MAX_Q, std::max<uint64_t>(32, up(2 * mean, 32))));
-    pair = mean > 112;
+    // Pairs where groups average many queries and many rows: else their fewer, taller tiles leave the groups' and the
+    // SMs' last rounds emptier than cheaper loads make up for. Without and with pairs, to bf16, groups x 2048 x 2048:
+    // mean 128 59.8 and 66.0 us, 256 49.5 and 52.1, 512 81.1 and 78.5, 1024 73.3 and 68.7; 8 x 4096 x 2048, mean 2048
+    // 136.7 and 128.2; 500 x 1000 x 128, mean 200 64 and 74; 32 x 300 x 512, mean 1024 19.1 and 23.3; 32 x 256 x 2048,
+    // mean 512 21.2 and 21.3; 64 x 700 x 300, mean 625 35.4 and 33.5.
+    pair = mean >= 512 && b.rows / g.groups > 512;
     p.subs = 1;
   }
   const uint32_t tile_rows = pair ? 2 * BM : p.subs * BM;

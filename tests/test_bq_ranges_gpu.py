@@ -223,3 +223,28 @@ def test_the_first_calls_of_a_context_may_be_captured():
     bq.check()
     del graph
     ctx.close()
+
+
+# ---- groups of many queries ----
+@pytest.mark.parametrize("mq,mb,dim", [
+    ([900], [600], 200),
+    ([600, 512, 700], [513, 600, 900], 130),
+    ([3000, 0, 5, 1], [200, 3000, 1, 77], 96),  # one group holds nearly all
+    ([800] * 7, [128] * 7, 64),  # no more rows than one CTA takes
+    ([4000, 1, 600, 0, 17], [1, 1700, 0, 128, 900], 520),
+    ([256] * 9, [300] * 9, 256),
+    ([513] * 4, [516] * 4, 300),
+])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_groups_of_many_queries_are_exact(mq, mb, dim, kind):
+    qo, bo = np.concatenate([[0], np.cumsum(mq)]), np.concatenate([[0], np.cumsum(mb)])
+    q, qv = whole_codes(int(qo[-1]), dim, 16)
+    b, bv = whole_codes(int(bo[-1]), dim, 17)
+    parts = [qv[qo[g]:qo[g + 1]] @ bv[bo[g]:bo[g + 1]].t() for g in range(len(mq))]
+    want = torch.cat([p.reshape(-1) for p in parts]).to(DTYPES[kind])
+    tq, tb = torch.from_numpy(qo).cuda(), torch.from_numpy(bo).cuda()
+    got = BlockQuantizer(dim).grouped_product(q, tq, b, tb, out_size=len(want), dtype=DTYPES[kind])
+    assert torch.equal(got, want)
+    if len(set(mb)) == 1:
+        even = BlockQuantizer(dim).grouped_product(q, tq, b, dtype=DTYPES[kind])
+        assert torch.equal(even.reshape(-1), want)
