@@ -18,8 +18,9 @@ static uint64_t up(uint64_t x, uint64_t to) { return (x + to - 1) / to * to; }
 static uint32_t blocks_of(uint32_t dim) { return (dim + BLOCK - 1) / BLOCK; }
 
 // ---- encode and decode ----
-// Both should be bound by the bytes they read and write, which leaves some 25 instructions of a warp per
-// block of 128. So eight lanes share a block and a warp works on four rows at once: a lane
+// Both should be bound by the bytes they read and write: a block of 16-bit components moves 388, which an SM's share of
+// 6.5 TB/s brings in 17 cycles, and its four schedulers issue 66 instructions of a warp meanwhile at the very
+// best. So eight lanes share a block and a warp works on four rows at once: a lane
 // moves 16 bytes of vector at a time, and what is done once per block (the reduction, the scale, the
 // addresses) is done for four. Items go by a fixed step: no division stands in the loop.
 //
@@ -489,9 +490,12 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr uint32_t F = FULL<T>;
     const bool wide = rows_wide(out, stride, dtype), few = dim <= SHORT_DIM<T>;
-    // Short rows leave the narrow kernel's warps part empty (1M x 31 f32: 92 us, as one array 42 us); long ones
-    // suit it (100003 x 1001 bf16: 75 us, as one array 79 us).
-    if (!wide && stride == dim && dim >= CHUNK<T> && blocks <= 2 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    // Short rows leave the narrow kernel's warps part empty; long ones suit it, 32-bit rows of two blocks already.
+    // Narrow and as one array, 2M rows of 31: f32 175 and 79 us, f16 178 and 54. 128M values of f32: dim 97 176 and 153,
+    // 127 157 and 151, 129 147 and 155, 193 140 and 149, 385 138 and 147, 1001 139 and 145; of f16: 129 143 and 108,
+    // 193 112 and 106, 257 111 and 106, 385 101 and 103, 1001 100 and 100.
+    constexpr uint32_t SHORT_BLOCKS = sizeof(T) == 4 ? 1 : 2;
+    if (!wide && stride == dim && dim >= CHUNK<T> && blocks <= SHORT_BLOCKS && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
       const uint64_t threads = (in.rows * dim + CHUNK<T> - 1) / CHUNK<T>;
       const unsigned grid =
           static_cast<unsigned>(std::min<uint64_t>((threads + 255) / 256, static_cast<uint64_t>(ctx->sm_count) * 32));
@@ -510,7 +514,10 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
 }
 
 // Several times 128 rows per tile where few queries leave a tile little work, as long as the rounds of
-// tiles over the SMs stay about as even.
+// tiles over the SMs stay about as even. By 128, 256 and 512 rows: 1 x 1M x 128 44.2, 31.4 and 31.2 us; 16 x 500k x 768
+// 76.0, 72.4 and 71.2; 48 x 100k x 768 20.6, 16.8 and 18.9; by 128 and 256: 64 x 100k x 768 20.9 and 16.8, 64 x 1M x 128
+// 77.2 and 78.0, 100 x 100k x 768 22.9 and 22.1. The rounds: 16 x 75,776 x 768 (four rounds by 128, one by 512) 14.8 and
+// 12.6; 1 x 20k x 768 (two and one) 10.6 and 10.7.
 static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, uint64_t sms) {
   const auto rounds = [&](uint64_t subs) { return up(up(rows, subs * bq_tc::BM) / (subs * bq_tc::BM), sms) / sms * subs; };
   for (uint32_t subs = q_rows <= 48 ? 4 : q_rows <= 64 ? 2 : 1; subs > 1; subs /= 2)
