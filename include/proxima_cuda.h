@@ -804,7 +804,10 @@ pxc_status pxc_bq_decode(pxc_ctx* ctx, const pxc_bq_rows* rows, uint32_t dim, vo
 pxc_status pxc_bq_decode_device(pxc_ctx* ctx, const pxc_bq_rows* d_rows, uint32_t dim, void* d_out, int32_t dtype,
                                 uint64_t stride, void* stream, pxc_error* err);
 /* The dot product of every pair of encoded rows: out[q * stride + r] = queries[q] .
- * base[r], summed in f32 and rounded once to `dtype`; stride >= base->rows. HOST buffers. */
+ * base[r], summed in f32 on the tensor cores and rounded once to `dtype`; stride >= base->rows.
+ * A sum is exact wherever 24 bits hold every partial one; else small terms are cut off
+ * where they are aligned with large ones (errors of 1.1 to 1.8 times those of plain f32
+ * sums measured, growing with dim). HOST buffers. */
 pxc_status pxc_bq_product(pxc_ctx* ctx, const pxc_bq_rows* queries, const pxc_bq_rows* base, uint32_t dim, void* out,
                           int32_t dtype, uint64_t stride, pxc_error* err);
 /* Same with DEVICE buffers. */

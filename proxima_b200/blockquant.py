@@ -6,7 +6,7 @@ It stands beside ``ScalarQuantizer`` (ranges per component) and ``ProductQuantiz
 each vector, so vectors of any distribution can be encoded as they arrive::
 
     bq = BlockQuantizer(768)
-    base = bq.encode(vectors)                      # BlockCodes: 1 byte a component + 1 a block
+    base = bq.encode(vectors)                      # BlockCodes: 1 byte a component + 1 a block (padded to 4 a row)
     scores = bq.product(bq.encode(queries), base)  # (nq, n) dot products, f32 sums
 
 ``grouped_product`` pairs ragged groups of queries with ragged groups of rows: the queries
@@ -238,7 +238,8 @@ class BlockQuantizer:
             codes = t.empty(n, ld, dtype=t.uint8, device=v.device)
             scales = codes.new_empty(n, sld)
             rows = N.PxcBqRows(codes.data_ptr(), scales.data_ptr(), n, ld, sld)
-            t.encode(self.ctx.handle, self._caller, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows), stream)
+            t.encode(self.ctx.handle, self._caller, v.data_ptr(), code, row if n > 1 else dim, dim, C.byref(rows),
+                     stream)
             return BlockCodes(codes, scales, dim)
         v = np.ascontiguousarray(v)
         codes, scales = np.zeros((n, ld), np.uint8), np.zeros((n, sld), np.uint8)
@@ -266,8 +267,9 @@ class BlockQuantizer:
 
     # -- products --
     def product(self, queries: BlockCodes, base: BlockCodes, dtype=None, out=None):
-        """The dot product of every pair of rows, (nq, n): f32 sums, rounded once to ``dtype``
-        (float32). ``out`` may be a tensor to write into, its rows strided."""
+        """The dot product of every pair of rows, (nq, n): f32 sums of the tensor cores (errors of 1.1 to 1.8
+        times those of plain f32 sums measured), rounded once to ``dtype`` (float32). ``out`` may be a
+        tensor to write into, its rows strided."""
         cuda = _is_cuda(queries.codes)
         q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base")
         shape = (q.rows, b.rows)
@@ -302,9 +304,9 @@ class BlockQuantizer:
         ``base[base_offsets[g]:base_offsets[g + 1]]``; either may be empty.
 
         Without ``base_offsets`` every group has len(base) / groups rows and the result is
-        (nq, rows); rows of queries in no group are not written. With them the result is flat: the groups'
-        matrices one after the other. ``out_size`` is its length (for tensors, reading the
-        offsets back to find it waits for the device)."""
+        (nq, rows); rows of queries in no group are not written (undefined in a tensor, 0 in an
+        array). With them the result is flat: the groups' matrices one after the other. ``out_size`` is its
+        length (for tensors, reading the offsets back to find it waits for the device)."""
         cuda = _is_cuda(queries.codes)
         dev = queries.codes.device if cuda else None
         q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base")

@@ -495,7 +495,8 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
     // 127 157 and 151, 129 147 and 155, 193 140 and 149, 385 138 and 147, 1001 139 and 145; of f16: 129 143 and 108,
     // 193 112 and 106, 257 111 and 106, 385 101 and 103, 1001 100 and 100.
     constexpr uint32_t SHORT_BLOCKS = sizeof(T) == 4 ? 1 : 2;
-    if (!wide && stride == dim && dim >= CHUNK<T> && blocks <= SHORT_BLOCKS && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    const bool flat = !wide && stride == dim && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    if (flat && dim >= CHUNK<T> && blocks <= SHORT_BLOCKS) {
       const uint64_t threads = (in.rows * dim + CHUNK<T> - 1) / CHUNK<T>;
       const unsigned grid =
           static_cast<unsigned>(std::min<uint64_t>((threads + 255) / 256, static_cast<uint64_t>(ctx->sm_count) * 32));
@@ -514,10 +515,10 @@ static void decode(pxc_ctx* ctx, const pxc_bq_rows& in, uint32_t dim, void* out,
 }
 
 // Several times 128 rows per tile where few queries leave a tile little work, as long as the rounds of
-// tiles over the SMs stay about as even. By 128, 256 and 512 rows: 1 x 1M x 128 44.2, 31.4 and 31.2 us; 16 x 500k x 768
-// 76.0, 72.4 and 71.2; 48 x 100k x 768 20.6, 16.8 and 18.9; by 128 and 256: 64 x 100k x 768 20.9 and 16.8, 64 x 1M x 128
-// 77.2 and 78.0, 100 x 100k x 768 22.9 and 22.1. The rounds: 16 x 75,776 x 768 (four rounds by 128, one by 512) 14.8 and
-// 12.6; 1 x 20k x 768 (two and one) 10.6 and 10.7.
+// tiles over the SMs stay about as even. By 128, 256 and 512 rows, queries' encoding not counted: 1 x 1M x 128 44.2, 31.4
+// and 31.2 us; 16 x 500k x 768 76.0, 72.4 and 71.2; 16 x 75,776 x 768 (4, 2 and 1 rounds) 14.8, 12.7 and 12.6; 1 x 20k x
+// 768 (2, 1 and 1) 10.6, 10.1 and 10.7; 48 x 100k x 768 20.6, 16.8 and 18.9. By 128 and 256: 64 x 100k x 768 20.9 and
+// 16.8, 64 x 1M x 128 77.2 and 78.0, 100 x 100k x 768 22.9 and 22.1.
 static uint32_t narrow_subs(uint32_t q_rows, uint64_t rows, uint64_t sms) {
   const auto rounds = [&](uint64_t subs) { return up(up(rows, subs * bq_tc::BM) / (subs * bq_tc::BM), sms) / sms * subs; };
   for (uint32_t subs = q_rows <= 48 ? 4 : q_rows <= 64 ? 2 : 1; subs > 1; subs /= 2)
