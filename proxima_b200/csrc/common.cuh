@@ -181,18 +181,16 @@ struct pxc_ctx {
 };
 
 namespace pxc {
-// RAII device selection. A thread's first CUDA call may be a driver one (the encoding of a tensor map), which wants
-// the device's context bound to the thread: naming the device binds it, even where it is the current one already.
+// RAII device selection.
 struct DeviceGuard {
+  const int device;
   int prev = -1;
-  explicit DeviceGuard(int dev) {
+  explicit DeviceGuard(int dev) : device(dev) {
     cudaGetDevice(&prev);
-    PXC_CUDA(cudaSetDevice(dev));
+    if (prev != dev) PXC_CUDA(cudaSetDevice(dev));
   }
   ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+    if (prev >= 0 && prev != device) cudaSetDevice(prev);
   }
 };
 
