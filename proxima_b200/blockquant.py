@@ -185,7 +185,7 @@ class BlockQuantizer:
         if codes.ndim != 2 or scales.ndim != 2:
             raise Configuration(name, 0, "codes and scales are uint8, one row per vector")
         if cuda:
-            byte, where, p, s = _torch().uint8, self.ctx.device, codes.data_ptr(), scales.data_ptr()
+            byte, where, p, s = (_torch_parts or _torch()).uint8, self.ctx.device, codes.data_ptr(), scales.data_ptr()
             (cr, cs), (sr, ss) = codes.stride(), scales.stride()
             if codes.get_device() != where or scales.get_device() != where:
                 raise Configuration("device", codes.get_device(), f"the context is on device {where}")
@@ -226,7 +226,7 @@ class BlockQuantizer:
         v = self._vectors(vectors)
         n, dim, ld, sld = len(v), self.dim, self._ld, self._sld
         if _is_cuda(v):
-            t = _torch()
+            t = _torch_parts or _torch()
             code = _codes.get(v.dtype)
             if code is None:
                 code = _dtype_code(v.dtype)
@@ -252,7 +252,7 @@ class BlockQuantizer:
         cuda = _is_cuda(codes.codes)
         rows = self._rows(codes, cuda, "codes")
         if cuda:
-            t = _torch()
+            t = _torch_parts or _torch()
             dtype = dtype or t.float32
             code = _codes.get(dtype)
             if code is None:
@@ -274,7 +274,7 @@ class BlockQuantizer:
         q, b = self._rows(queries, cuda, "queries"), self._rows(base, cuda, "base")
         shape = (q.rows, b.rows)
         if cuda:
-            t, dev = _torch(), queries.codes.device
+            t, dev = _torch_parts or _torch(), queries.codes.device
             stride = shape[1] or 1
             if out is None:
                 dtype = dtype or t.float32
@@ -327,7 +327,7 @@ class BlockQuantizer:
             size = int(out_size)
             shape = (size,)
         if cuda:
-            t = _torch()
+            t = _torch_parts or _torch()
             dtype = dtype or t.float32
             code = _codes.get(dtype)
             if code is None:
@@ -347,7 +347,7 @@ class BlockQuantizer:
         if not cuda and _is_cuda(o):
             raise Configuration("offsets", 0, "all operands on one device, or all on the host")
         if cuda:
-            if not _is_cuda(o) or o.device != dev or o.dtype != _torch().int64 or o.ndim != 1:
+            if not _is_cuda(o) or o.device != dev or o.dtype != (_torch_parts or _torch()).int64 or o.ndim != 1:
                 raise Configuration("offsets", 0, "must be an int64 tensor on the operands' device")
             return o.contiguous()
         o = np.asarray(o)

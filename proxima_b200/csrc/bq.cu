@@ -394,15 +394,17 @@ struct Caller {
     Reports& reports = *ctx->bq_reports;
     if (number != 0) {
       told[0] = record = reports.of_caller(number, fails);
+      if (fails && capturing()) reports.keep(number);
       return;
     }
     told[0] = record = reports.of_stream(stream);
     told[1] = reports.captured();
+    if (fails && capturing()) record = reports.captured();
+  }
+  bool capturing() const {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess)
-      cudaGetLastError();  // the launch will say what is wrong
-    else if (status != cudaStreamCaptureStatusNone)
-      record = reports.captured();
+    if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) cudaGetLastError();  // the launch will say what is wrong
+    return status != cudaStreamCaptureStatusNone;
   }
   void report() const {
     for (const Record& r : told)

@@ -4,12 +4,14 @@
 // write into them. Callers are those that name themselves by a number, the streams of calls made without one, and
 // each host call. Ids are never used twice, so a kernel or graph that outlives its caller is not taken for
 // another's, and the words stay allocated until the context goes. A record whose caller has gone is given out again
-// late, behind at least QUARANTINE others; what its work leaves meanwhile is for whoever checks.
+// late, behind at least QUARANTINE others, or never if a graph may hold its calls; what its work leaves is for
+// whoever checks.
 #pragma once
 
 #include <deque>
 #include <mutex>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "common.cuh"
@@ -74,12 +76,20 @@ class Reports {
     Record& r = callers_[caller];
     return r = take_slot();
   }
+  // The caller's graphs may run whenever, also once it has gone.
+  void keep(uint64_t caller) {
+    std::lock_guard<std::mutex> lock(mu_);
+    kept_.insert(caller);
+  }
   void forget(const uint64_t* callers, uint64_t count) {
     std::lock_guard<std::mutex> lock(mu_);
     for (uint64_t i = 0; i < count; ++i) {
       const auto found = callers_.find(callers[i]);
       if (found == callers_.end()) continue;
-      free_.push_back(found->second);
+      if (kept_.erase(callers[i]))
+        of_graphs_.push_back(found->second);
+      else
+        free_.push_back(found->second);
       callers_.erase(found);
     }
   }
@@ -87,6 +97,7 @@ class Reports {
   void take_left() {
     std::lock_guard<std::mutex> lock(mu_);
     for (const Record& r : free_) r.take();
+    for (const Record& r : of_graphs_) r.take();
     for (const Fault f : {FAULT_TIMEOUT, FAULT_OFFSETS})
       if (left_[f]) {
         left_[f] = false;
@@ -139,6 +150,8 @@ class Reports {
   std::deque<Record> free_;  // with the ids of callers who have gone
   bool left_[FAULT_WORDS] = {};  // failures found in a record that was given out again
   std::unordered_map<uint64_t, Record> callers_;
+  std::unordered_set<uint64_t> kept_;  // those of them that a graph may hold calls of
+  std::vector<Record> of_graphs_;      // and the records of such callers who have gone
   std::unordered_map<const void*, Record> streams_;
   Record captured_;
   uint32_t last_id_ = 0;

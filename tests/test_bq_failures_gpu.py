@@ -279,6 +279,8 @@ def test_failures_of_quantisers_that_are_gone(ctx):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         BlockQuantizer(48, context=ctx).grouped_product(q, off, base)
+    for _ in range(1500):  # more than there are records before they are given out again
+        BlockQuantizer(48, context=ctx).product(q, base)
     off.copy_(torch.tensor(BAD))
     kept.check()
     graph.replay()
